@@ -170,7 +170,8 @@ size_t oc_b200_gptq_gemm_workspace(const oc_b200_layer* layer, int64_t M);
 int oc_b200_gptq_gemm(const oc_b200_layer* layer, const void* a, int a_dtype, int64_t M, int64_t lda,
                       const void* bias, int bias_dtype, void* c, int64_t ldc, void* workspace,
                       size_t workspace_bytes, oc_stream_t stream);
-enum { OC_ACT_NONE = 0, OC_ACT_GELU_TANH = 1 };
+/* OC_ACT_GELU (erf), OC_ACT_SILU and OC_ACT_RELU: oc_b200_dense_gemm only */
+enum { OC_ACT_NONE = 0, OC_ACT_GELU_TANH = 1, OC_ACT_GELU = 2, OC_ACT_SILU = 3, OC_ACT_RELU = 4 };
 /* oc_b200_gptq_gemm with a fused epilogue: C = act(A @ W^T + bias) + residual, evaluated in
  * fp32 and rounded once (act: OC_ACT_NONE or OC_ACT_GELU_TANH, torch's approximate="tanh";
  * residual: optional [M, ldr] in a_dtype, may alias C). Folds the activation and residual
@@ -294,6 +295,46 @@ int oc_b200_nvls_allreduce_bf16(void* mc_ptr, int64_t n_elems, void* const* flag
 int oc_b200_nvls_allreduce_rmsnorm_bf16(void* mc_ptr, int rows, int cols, const void* gain, float eps,
                                         void* const* flags_dev, int rank, int world, uint32_t epoch, int blocks,
                                         oc_stream_t stream);
+
+/* ---- transformer-block operators beside the packed linears -------------------
+ * No reference counterpart (the reference leaves them to torch). All are stream-ordered, allocate
+ * nothing and run on the current device.
+ *
+ * Rotary positions. Tensors are [T, H, D] (dtype f16, bf16 or f32), token and head strides in
+ * elements, unit stride inside a head; k may be absent (Hk = 0). The first R of D values (R even) are
+ * rotated: pairs (i, i + R/2), or (2i, 2i + 1) if interleaved; pair i turns by
+ * position * turns[i] / 2^64 of a full turn and is multiplied by gain. positions: int32 or int64
+ * [T, axes], rows positions_st elements apart; axis[i] picks pair i's column (NULL: column 0, and
+ * every axis[i] must be a column). turns, axis: device arrays of R/2. q_out / k_out may be the inputs;
+ * out of place the D - R values behind the rotated part are copied. */
+int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int Hq,
+                 const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int Hk,
+                 int dtype, int T, int D, int R, const void* positions, int positions_64, int64_t positions_st,
+                 const uint64_t* turns, const uint8_t* axis, float gain, int interleaved, oc_stream_t stream);
+/* Attention over packed sequences: out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G]) v[j, h / G],
+ * G = Hq / Hkv, over the keys of row i's sequence (f16 or bf16, fp32 softmax and sums). q, out:
+ * [Tq, Hq, D]; k, v: [Tk, Hkv, D]; token and head strides in elements, multiples of 8, tensors
+ * 16-byte aligned, D a multiple of 8 up to 256. Sequence b: query rows cu_q[b] .. cu_q[b+1], key rows
+ * from cu_k[b], kv_lens[b] of them (NULL: up to cu_k[b+1]); cu_q = cu_k = NULL: one sequence of all
+ * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros.
+ * Query rows outside every sequence stay as they were, or become zeros with zero_tail (rows behind
+ * cu_q[B]). The tables are read on the device; values outside the tensors are clamped and set the
+ * device error word. max_q (0: unknown) is a hint of the longest query run; it only picks a kernel.
+ * workspace: oc_b200_attention_workspace(D) bytes on the current device, any contents, 16-byte
+ * aligned, not shared by calls that may run at once. out must not overlap the inputs. */
+size_t oc_b200_attention_workspace(int D);
+int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                      const void* v, int64_t v_st, int64_t v_sh, void* out, int64_t o_st, int64_t o_sh, int dtype,
+                      int Tq, int Tk, int Hq, int Hkv, int D, const int32_t* cu_q, const int32_t* cu_k,
+                      const int32_t* kv_lens, int B, int causal, float scale, int max_q, int zero_tail,
+                      void* workspace, size_t workspace_bytes, oc_stream_t stream);
+/* Dense linear: C[M, N] = act(X[M, K] W[N, K]^T + bias) + residual, f16 or bf16 with fp32
+ * accumulation and epilogue, one rounding. K a multiple of 8, X and W rows 16-byte aligned; bias
+ * [N] f16, bf16 or f32 or NULL; residual [M, ldr] or NULL, may be C itself; C and residual rows of any
+ * alignment. */
+int oc_b200_dense_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int M, int N, int K,
+                       const void* bias, int bias_dtype, const void* residual, int64_t ldr, int act, void* c,
+                       int64_t ldc, oc_stream_t stream);
 
 #ifdef __cplusplus
 }

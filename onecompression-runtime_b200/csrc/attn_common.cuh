@@ -1,0 +1,87 @@
+// Attention over packed sequences: what the kernels share.
+//
+// Sequence b owns the query rows [cu_q[b], cu_q[b+1]) and the key rows that start at cu_k[b]; it
+// sees kv_lens[b] of them, or all up to cu_k[b+1]. With causal masking the last query sees the last
+// key: query i of nq sees the keys j <= i + nk - nq. A row that sees no key gives zeros.
+// The tables live on the device and are clamped to the tensors here, so no table value can send an
+// access out of range; a clamped value sets the device error word.
+#pragma once
+
+#include "common.cuh"
+
+namespace oc {
+
+struct AttnParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;  // token and head strides (elements)
+  int Tq, Tk, Hq, Hkv, G, D;                                 // G = Hq / Hkv
+  const int* cu_q;      // [B + 1] or null: one sequence over all rows
+  const int* cu_k;
+  const int* kv_lens;   // [B] or null
+  int B;
+  int causal;
+  int zero_tail;        // also write zeros to the query rows that no sequence owns
+  float scale_log2;     // softmax scale * log2(e)
+  float* part;          // split kernel: partial results
+  int* desc;            // split kernel: one descriptor per CTA
+};
+
+struct Seq { int q0, nq, k0, nk; };
+
+__device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report = false) {
+  int q0 = 0, q1 = p.Tq, k0 = 0, k1 = p.Tk;
+  if (p.cu_q) { q0 = p.cu_q[b]; q1 = p.cu_q[b + 1]; }
+  if (p.cu_k) { k0 = p.cu_k[b]; k1 = p.cu_k[b + 1]; }
+  Seq s;
+  s.q0 = min(max(q0, 0), p.Tq);
+  const int qe = min(max(q1, s.q0), p.Tq);
+  s.k0 = min(max(k0, 0), p.Tk);
+  const int ke = min(max(k1, s.k0), p.Tk);
+  s.nq = qe - s.q0;
+  s.nk = ke - s.k0;
+  bool bad = s.q0 != q0 || qe != q1 || s.k0 != k0 || ke != k1;
+  if (p.kv_lens) {
+    const int n = p.kv_lens[b];
+    bad |= n < 0 || n > s.nk;
+    s.nk = min(max(n, 0), s.nk);
+  }
+  if (report && bad) record_error(kDevErrSeq);
+  return s;
+}
+
+// The first query row behind the last sequence.
+__device__ __forceinline__ int attn_tail(const AttnParams& p) {
+  return p.cu_q ? min(max(p.cu_q[p.B], 0), p.Tq) : p.Tq;
+}
+
+// One CTA's share of the rows that no sequence owns: zeros (D is a multiple of 8, rows 16-byte aligned).
+__device__ __forceinline__ void attn_zero_tail(const AttnParams& p, int cta, int n_ctas) {
+  const int vecs = p.D / 8;
+  for (long long t = (long long)attn_tail(p) + cta; t < p.Tq; t += n_ctas)
+    for (int i = threadIdx.x; i < p.Hq * vecs; i += blockDim.x)
+      *reinterpret_cast<uint4*>(p.out + t * p.o_st + (i / vecs) * p.o_sh + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Is one of the two 16-bit values of a register infinite or NaN?
+template <bool BF16> __device__ __forceinline__ bool nonfinite2(uint32_t v) {
+  constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;
+  return (v & m) == m || ((v >> 16) & m) == m;
+}
+// The register with infinite and NaN halves set to zero.
+template <bool BF16> __device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;
+  if ((v & m) == m) v &= 0xFFFF0000u;
+  if (((v >> 16) & m) == m) v &= 0x0000FFFFu;
+  return v;
+}
+
+}  // namespace oc

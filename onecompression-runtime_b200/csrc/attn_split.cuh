@@ -1,0 +1,383 @@
+// Attention for few query rows per sequence: single tokens, short runs of tokens, short prompts.
+//
+// Bound by HBM: one pass over the keys and values. The (token, head) rows of one key head are packed
+// into tiles of 16 rows, so a group of query heads shares every key it reads. The work of a call is
+// the list of 64-key blocks of all (sequence, key head, row tile) items in order; the CTAs of one
+// full wave take equal runs of that list, found on the device from the length tables, so ragged
+// lengths and long caches spread over every SM without the host knowing a length. Inside a run
+// four warps take 16-key slices in turn, each through a private cp.async ring (no CTA barrier while
+// streaming), with m16n8k16 tensor-core products, the running row maximum and sum in fp32 and base 2
+// exponents. The warps are joined through shared memory; an item that spans CTAs leaves fp32
+// partials (maximum, sum, unnormalized output) that attn_join_kernel adds in CTA order: no atomics,
+// the same bits on every run.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace oc {
+
+constexpr int kSplitWarps = 4;
+constexpr int kSplitThreads = kSplitWarps * 32;
+constexpr int kSplitRows = 16;      // rows of a tile
+constexpr int kSplitBlock = 64;     // keys of a work unit
+constexpr int kSplitDescInts = 8;
+
+template <int DP> struct SplitCfg {
+  static constexpr int kKvBytes = 16 * DP * 2;                 // 16 keys (or values)
+  static constexpr int kStageBytes = 2 * kKvBytes;
+  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
+  static constexpr int kRingBytes = kSplitWarps * kStages * kStageBytes;   // 96 KB; 192 KB at DP = 256
+  static constexpr int kPitch = DP + 8;                        // floats of a joined row
+  static constexpr int kPartFloats = kSplitRows * (DP + 2);    // one partial: O [16][DP], m [16], l [16]
+  static_assert(kSplitWarps * kSplitRows * kPitch * 4 <= kRingBytes, "the warps' outputs fit the ring");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Work units of a sequence: key heads x row tiles x 64-key blocks (one block where no key is).
+__device__ __forceinline__ int split_blocks(int nk) { return nk > 0 ? (nk + kSplitBlock - 1) / kSplitBlock : 1; }
+__device__ __forceinline__ long long split_tiles(const AttnParams& p, int nq) {
+  return ((long long)nq * p.G + kSplitRows - 1) / kSplitRows;
+}
+__device__ __forceinline__ long long split_units(const AttnParams& p, const Seq& s) {
+  return (long long)p.Hkv * split_tiles(p, s.nq) * split_blocks(s.nk);
+}
+
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_split_kernel(const AttnParams p) {
+  using Cfg = SplitCfg<DP>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sm_m[kSplitWarps][kSplitRows], sm_l[kSplitWarps][kSplitRows];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = warp_id(), lane = lane_id();
+  const int g = lane >> 2, tq = lane & 3;
+  int* desc = p.desc + blockIdx.x * kSplitDescInts;
+  if (threadIdx.x == 0) desc[0] = 0;   // rows of the item this CTA begins and others finish
+
+  // the call's units, then this CTA's run of them (every warp finds it for itself)
+  long long total = 0;
+  for (int base = 0; base < p.B; base += 32) {
+    long long u = 0;
+    if (base + lane < p.B) u = split_units(p, attn_seq(p, base + lane, blockIdx.x == 0 && warp == 0));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    total += u;
+  }
+  if (p.zero_tail) attn_zero_tail(p, blockIdx.x, gridDim.x);
+  const long long n = total < (long long)gridDim.x ? total : (long long)gridDim.x;
+  if (blockIdx.x >= n) return;
+  const long long u_end = total * (blockIdx.x + 1) / n;
+  long long u = total * blockIdx.x / n;
+  int b = 0;
+  long long seq_begin = 0;   // first unit of sequence b
+  for (int base = 0; base < p.B; base += 32) {
+    long long mine = 0;
+    if (base + lane < p.B) mine = split_units(p, attn_seq(p, base + lane));
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base + lane < p.B && seq_begin + incl > u);
+    if (past) {
+      const int f = __ffs(past) - 1;
+      b = base + f;
+      seq_begin += __shfl_sync(0xffffffffu, incl - mine, f);
+      break;
+    }
+    seq_begin += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  Seq s = attn_seq(p, b);
+
+  uint8_t* ring = smem + warp * (Cfg::kStages * Cfg::kStageBytes);
+  const uint32_t ring_addr = smem_u32(ring);
+  constexpr int kCh = DP / 8;                      // 16-byte chunks of a row
+  constexpr int kIter = 16 * kCh / 32;             // chunks per lane of one 16-row matrix
+
+  while (u < u_end) {
+    while (u >= seq_begin + split_units(p, s)) {
+      seq_begin += split_units(p, s);
+      s = attn_seq(p, ++b);
+    }
+    const int nblk = split_blocks(s.nk);
+    const long long rel = u - seq_begin;
+    const long long item = rel / nblk;
+    const int blk0 = (int)(rel - item * nblk);
+    const int blk1 = (int)min((long long)nblk, blk0 + (u_end - u));
+    const long long tiles = split_tiles(p, s.nq);
+    const int kvh = (int)(item / tiles);
+    const long long row0 = (item - kvh * tiles) * kSplitRows;
+    const int rows = (int)min((long long)kSplitRows, (long long)s.nq * p.G - row0);
+    const int kbeg = blk0 * kSplitBlock, kend = min(s.nk, blk1 * kSplitBlock);
+
+    // this lane's two rows: last visible key, and the queries as A fragments
+    int limit[2];
+    uint32_t qa[DP / 16][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = g + 8 * i;
+      const long long row = row0 + r;
+      const int tok = (int)(row / p.G);
+      const uint16_t* qr = p.q + (s.q0 + tok) * p.q_st + (kvh * p.G + row % p.G) * p.q_sh;
+      limit[i] = r < rows ? (p.causal ? min(kend - 1, tok + s.nk - s.nq) : kend - 1) : -1;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = ks * 16 + h * 8 + 2 * tq;
+          qa[ks][2 * h + i] = (r < rows && col < p.D) ? *reinterpret_cast<const uint32_t*>(qr + col) : 0u;
+        }
+    }
+    const int first_limit = p.causal ? (int)(row0 / p.G) + s.nk - s.nq : kend - 1;   // of the tile's first token
+
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    const uint16_t* kb = p.k + s.k0 * p.k_st + kvh * p.k_sh;
+    const uint16_t* vb = p.v + s.k0 * p.v_st + kvh * p.v_sh;
+    const int slices = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
+    // rows behind the last key and columns behind D are filled with zeros: a weight of zero times
+    // whatever lies there must not reach the output
+    auto issue = [&](int sl, int stage) {
+      if (sl < slices) {
+        const int key0 = kbeg + sl * 16;
+        const uint32_t dst = ring_addr + stage * Cfg::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) {
+          const int idx = i * 32 + lane, r = idx / kCh, ch = idx % kCh;
+          const bool ok = key0 + r < kend && ch * 8 < p.D;
+          const long long key = ok ? key0 + r : 0;
+          const int col = ok ? ch * 8 : 0;
+          const uint32_t off = dst + r * (DP * 2) + ((ch ^ (r & 7)) * 16);
+          cp_async16(off, (ok ? kb + key * p.k_st + col : p.k), ok);
+          cp_async16(off + Cfg::kKvBytes, (ok ? vb + key * p.v_st + col : p.v), ok);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < Cfg::kStages - 1; ++i) issue(warp + i * kSplitWarps, i);
+    int stage = 0;
+    for (int sl = warp; sl < slices; sl += kSplitWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 2) : "memory");
+      __syncwarp();   // every lane's copies of this stage have landed; the stage refilled next is read
+      issue(sl + (Cfg::kStages - 1) * kSplitWarps, stage == 0 ? Cfg::kStages - 1 : stage - 1);
+      const uint32_t ks_addr = ring_addr + stage * Cfg::kStageBytes;
+      const uint32_t vs_addr = ks_addr + Cfg::kKvBytes;
+      const int key0 = kbeg + sl * 16;
+      float c[2][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        uint32_t r[4];
+        const int row = (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+        ldsm_x4(ks_addr + row * (DP * 2) + ((ch ^ (row & 7)) * 16), r);
+        mma16816<BF16>(c[0], qa[ks], r[0], r[1]);
+        mma16816<BF16>(c[1], qa[ks], r[2], r[3]);
+      }
+      float corr[2];
+      uint32_t pa[4];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = m[i];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = c[t][2 * i + e];
+            x = key0 + t * 8 + 2 * tq + e <= limit[i] ? x * p.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        corr[i] = ex2(m[i] - ref);
+        grew |= mx != m[i];
+        m[i] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float p0 = ex2(c[t][2 * i] - ref), p1 = ex2(c[t][2 * i + 1] - ref);
+          sum += p0 + p1;
+          pa[2 * t + i] = pack2_rn<BF16>(p0, p1);   // weights in [0, 1] as the product's 16-bit operand
+        }
+        l[i] = l[i] * corr[i] + sum;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+          o[i][0] *= corr[0]; o[i][1] *= corr[0];
+          o[i][2] *= corr[1]; o[i][3] *= corr[1];
+        }
+      }
+      // does a row of the tile see less than this slice? then a value it does not see may be
+      // infinite or NaN, and its weight of zero must not turn that into NaN
+      const bool edge = min(key0 + 15, kend - 1) > first_limit;
+#pragma unroll
+      for (int d2 = 0; d2 < DP / 16; ++d2) {
+        uint32_t r[4];
+        const int row = lane & 15, ch = d2 * 2 + (lane >> 4);
+        ldsm_x4_trans(vs_addr + row * (DP * 2) + ((ch ^ (row & 7)) * 16), r);
+        bool odd = false;
+        if (edge) {
+          odd = nonfinite2<BF16>(r[0]) || nonfinite2<BF16>(r[1]) || nonfinite2<BF16>(r[2]) || nonfinite2<BF16>(r[3]);
+          odd = __any_sync(0xffffffffu, odd);
+          if (odd)
+            for (int i = 0; i < 4; ++i) r[i] = finite2<BF16>(r[i]);
+        }
+        mma16816<BF16>(o[2 * d2], pa, r[0], r[1]);
+        mma16816<BF16>(o[2 * d2 + 1], pa, r[2], r[3]);
+        if (odd) {   // the rows that do see such a value add it
+          for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int col = d2 * 16 + t * 8 + 2 * tq + e;
+                const int cc = (col >> 3) ^ (j & 7);
+                const uint16_t bits = *reinterpret_cast<const uint16_t*>(
+                    smem + (vs_addr - smem_u32(smem)) + j * (DP * 2) + cc * 16 + (col & 7) * 2);
+                if (nonfinite2<BF16>(bits))
+#pragma unroll
+                  for (int i = 0; i < 2; ++i)
+                    if (key0 + j <= limit[i]) o[2 * d2 + t][2 * i + e] += bits_to_f32(bits, BF16 ? kBF16 : kF16);
+              }
+        }
+      }
+      stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();   // the rings are read; they now hold the warps' outputs
+
+    float* osm = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      float* orow = osm + (warp * kSplitRows + g + 8 * i) * Cfg::kPitch;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d)
+        *reinterpret_cast<float2*>(orow + d * 8 + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+      if (tq == 0) {
+        sm_m[warp][g + 8 * i] = m[i];
+        sm_l[warp][g + 8 * i] = l[i];
+      }
+    }
+    __syncthreads();
+    const bool whole = blk0 == 0 && blk1 == nblk;
+    float* part = p.part + ((long long)blockIdx.x * 2 + (blk0 == 0 ? 1 : 0)) * Cfg::kPartFloats;
+    for (int i = threadIdx.x; i < rows * (DP / 4); i += kSplitThreads) {
+      const int r = i / (DP / 4), c4 = (i % (DP / 4)) * 4;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kSplitWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      float lsum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kSplitWarps; ++w) {
+        const float a = ex2(sm_m[w][r] - ref);
+        const float4 x = *reinterpret_cast<const float4*>(osm + (w * kSplitRows + r) * Cfg::kPitch + c4);
+        lsum += a * sm_l[w][r];
+        acc.x += a * x.x; acc.y += a * x.y; acc.z += a * x.z; acc.w += a * x.w;
+      }
+      if (whole) {
+        if (c4 < p.D) {
+          const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+          const long long row = row0 + r;
+          uint16_t* dst = p.out + (s.q0 + row / p.G) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + c4;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_rn<BF16>(acc.x * inv, acc.y * inv),
+                                                      pack2_rn<BF16>(acc.z * inv, acc.w * inv));
+        }
+      } else {
+        *reinterpret_cast<float4*>(part + r * DP + c4) = acc;
+        if (c4 == 0) {
+          part[kSplitRows * DP + r] = mx;
+          part[kSplitRows * DP + kSplitRows + r] = lsum;
+        }
+      }
+    }
+    if (!whole && blk0 == 0 && threadIdx.x == 0) {
+      const long long last = seq_begin + (item + 1) * nblk - 1;   // the item's last unit
+      desc[1] = (int)(((last + 1) * n - 1) / total);              // the CTA that holds it
+      desc[2] = s.q0;
+      desc[3] = kvh;
+      *reinterpret_cast<long long*>(desc + 4) = row0;
+      desc[0] = rows;
+    }
+    __syncthreads();
+    u += blk1 - blk0;
+  }
+}
+
+// Joins the partials of the item that CTA blockIdx.x began: slot 1 of that CTA, slot 0 of the CTAs
+// after it up to the item's last one, in that order. One warp per row.
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+  using Cfg = SplitCfg<DP>;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int* desc = p.desc + blockIdx.x * kSplitDescInts;
+  const int r = blockIdx.y * 4 + warp_id(), lane = lane_id();
+  if (r >= desc[0]) return;
+  const int c0 = blockIdx.x, c1 = desc[1];
+  auto slot = [&](int c) { return p.part + ((long long)c * 2 + (c == c0 ? 1 : 0)) * Cfg::kPartFloats; };
+  float mx = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, slot(c)[kSplitRows * DP + r]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float lsum = 0.f;
+  constexpr int kV = DP / 32;   // columns of a lane
+  float acc[kV];
+#pragma unroll
+  for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float* s = slot(c);
+    const float a = ex2(s[kSplitRows * DP + r] - ref);
+    lsum += a * s[kSplitRows * DP + kSplitRows + r];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] += a * s[r * DP + lane * kV + i];
+  }
+  const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+  const long long row = *reinterpret_cast<const long long*>(desc + 4) + r;
+  uint16_t* dst = p.out + (desc[2] + row / p.G) * p.o_st + (desc[3] * p.G + row % p.G) * p.o_sh + lane * kV;
+  if (lane * kV < p.D) {
+#pragma unroll
+    for (int i = 0; i < kV; i += 2)
+      *reinterpret_cast<uint32_t*>(dst + i) = pack2_rn<BF16>(acc[i] * inv, acc[i + 1] * inv);
+  }
+}
+
+}  // namespace oc

@@ -1,0 +1,261 @@
+// C ABI of the operators between and beside the packed linears of a transformer block: rotary
+// positions, attention over packed sequences, the dense 16-bit linear.
+#include <climits>
+#include <cmath>
+
+#include "../../include/oc_b200.h"
+#include "common.cuh"
+#include "host.h"
+#include "rope.cuh"
+#include "attn_common.cuh"
+#include "attn_split.cuh"
+#include "gemm_dense.cuh"
+
+// This translation unit's device error word (common.cuh defines one per unit), for
+// oc_b200_read_device_error.
+int block_ops_device_error(unsigned* value, cudaStream_t stream) {
+  const unsigned zero = 0;
+  if (int rc = cuda_check(cudaMemcpyFromSymbolAsync(value, oc::g_oc_dev_error, sizeof(*value), 0,
+                                                    cudaMemcpyDeviceToHost, stream), "read device error"))
+    return rc;
+  return cuda_check(cudaMemcpyToSymbolAsync(oc::g_oc_dev_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream),
+                    "clear device error");
+}
+
+namespace {
+
+// Raises a kernel's dynamic shared memory limit: an attribute per device, so set on every launch.
+template <typename K> int set_smem(K kern, int bytes) {
+  return cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                    "shared memory limit");
+}
+
+// ------------------------------------------------------------------ rotary positions
+template <int DT, int V, bool INTER>
+int launch_rope(const oc::RopeParams& p0, int sms, cudaStream_t stream) {
+  oc::RopeParams p = p0;
+  const int heads = p.t[0].H + p.t[1].H;
+  // Four tokens to a block once that still gives every SM several blocks; below, one token, its heads
+  // spread over blocks until about two blocks per SM run.
+  const int tb = p.T >= 4 * 4 * sms ? 4 : 1;
+  const long long gx = ((long long)p.T + tb - 1) / tb;
+  long long want = gx >= 2 * sms ? 1 : (2 * sms + gx - 1) / gx;
+  if (want > heads) want = heads;
+  p.heads_per_block = (int)((heads + want - 1) / want);
+  const dim3 grid((unsigned)gx, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block));
+  const size_t smem = (size_t)tb * p.R * sizeof(float);
+  if (tb == 4)
+    oc::rope_kernel<DT, V, INTER, 4><<<grid, oc::kRopeThreads, smem, stream>>>(p);
+  else
+    oc::rope_kernel<DT, V, INTER, 1><<<grid, oc::kRopeThreads, smem, stream>>>(p);
+  return launch_check("rope");
+}
+
+template <int DT, int VMAX>
+int launch_rope_dt(const oc::RopeParams& p, bool vec, bool inter, int sms, cudaStream_t stream) {
+  if (vec) return inter ? launch_rope<DT, VMAX, true>(p, sms, stream) : launch_rope<DT, VMAX, false>(p, sms, stream);
+  return inter ? launch_rope<DT, 1, true>(p, sms, stream) : launch_rope<DT, 1, false>(p, sms, stream);
+}
+
+// ------------------------------------------------------------------ attention
+int attn_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+template <int DP> int split_ctas(int sms) { return sms * oc::SplitCfg<DP>::kCtasPerSm; }
+int split_ctas(int dp, int sms) {
+  return dp == 64 ? split_ctas<64>(sms) : dp == 128 ? split_ctas<128>(sms) : split_ctas<256>(sms);
+}
+size_t split_desc_bytes(int ctas) { return (((size_t)ctas * oc::kSplitDescInts * 4) + 255) / 256 * 256; }
+size_t split_ws_bytes(int dp, int ctas) {
+  return split_desc_bytes(ctas) + (size_t)ctas * 2 * oc::kSplitRows * (dp + 2) * 4;
+}
+
+template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas, cudaStream_t stream) {
+  auto kern = oc::attn_split_kernel<BF16, DP>;
+  if (int rc = set_smem(kern, oc::SplitCfg<DP>::kRingBytes)) return rc;
+  kern<<<ctas, oc::kSplitThreads, oc::SplitCfg<DP>::kRingBytes, stream>>>(p);
+  if (int rc = launch_check("attention (split)")) return rc;
+  return launch_pdl(oc::attn_join_kernel<BF16, DP>, dim3((unsigned)ctas, oc::kSplitRows / 4), dim3(128), 0, stream,
+                    "attention (join)", p);
+}
+
+// ------------------------------------------------------------------ dense linear
+template <bool BF16, int BN>
+int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, oc::DenseParams p, int dev,
+                       cudaStream_t stream) {
+  using Cfg = oc::DsCfg<BN>;
+  const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tw, tx;
+  if (int rc = make_tmap_2d(&tw, dt, 2, w, p.K, p.N, (uint64_t)ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tmap_2d(&tx, dt, 2, x, p.K, p.M, (uint64_t)ldx * 2, 64, BN, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  p.n_tiles_m = (p.M + BN - 1) / BN;
+  const long long tiles = (long long)((p.N + 127) / 128) * p.n_tiles_m;
+  const int slots = sm_count(dev) * (BN <= 64 ? 2 : 1);
+  const int kb = (p.K + 63) / 64;
+  int S = 1;
+  while (S < 8 && tiles * S * 2 <= slots && kb >= S * 2 * 2) S *= 2;
+  if (tiles * S > INT_MAX) return fail(OC_ERR_INVALID, "dense_gemm: %lld tiles", tiles);
+  auto kern = oc::dense_split_kernel<BF16, BN>;
+  if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * S));
+  cfg.blockDim = dim3(oc::kDsThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (int rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, tw, tx, p), "dense_gemm")) return rc;
+  return launch_check("dense_gemm");
+}
+
+template <bool BF16>
+int launch_dense(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& p, int dev,
+                 cudaStream_t stream) {
+  if (p.M <= 16) return launch_dense_split<BF16, 16>(x, ldx, w, ldw, p, dev, stream);
+  if (p.M <= 32) return launch_dense_split<BF16, 32>(x, ldx, w, ldw, p, dev, stream);
+  if (p.M <= 64) return launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream);
+  if (p.M <= 128) return launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
+  return launch_dense_split<BF16, 256>(x, ldx, w, ldw, p, dev, stream);
+}
+
+}  // namespace
+
+extern "C" int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                            int Hq, const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st,
+                            int64_t ko_sh, int Hk, int dtype, int T, int D, int R, const void* positions,
+                            int positions_64, int64_t positions_st, const uint64_t* turns, const uint8_t* axis,
+                            float gain, int interleaved, oc_stream_t stream_) {
+  if (T < 0 || Hq < 0 || Hk < 0 || D <= 0 || D > 1024 || R <= 0 || R > D || R % 2 != 0)
+    return fail(OC_ERR_INVALID, "rope: T=%d Hq=%d Hk=%d D=%d R=%d (R even, at most D; D at most 1024)", T, Hq, Hk, D, R);
+  if (!dtf(dtype)) return fail(OC_ERR_INVALID, "rope: dtype %d", dtype);
+  if (Hq > 65535 || Hk > 65535) return fail(OC_ERR_INVALID, "rope: %d + %d heads", Hq, Hk);
+  if (T == 0 || Hq + Hk == 0) return OC_OK;
+  if ((Hq && (!q || !q_out)) || (Hk && (!k || !k_out)) || !positions || !turns)
+    return fail(OC_ERR_INVALID, "rope: NULL pointer");
+  if (!std::isfinite(gain)) return fail(OC_ERR_INVALID, "rope: gain %g", (double)gain);
+  oc::RopeParams p{};
+  p.t[0] = {q, q_out, q_st, q_sh, qo_st, qo_sh, Hq};
+  p.t[1] = {k, k_out, k_st, k_sh, ko_st, ko_sh, Hk};
+  p.T = T;
+  p.D = D;
+  p.R = R;
+  p.pos = positions;
+  p.pos64 = positions_64;
+  p.pos_st = positions_st;
+  p.turns = reinterpret_cast<const unsigned long long*>(turns);
+  p.axis = axis;
+  p.gain = gain;
+  p.copy_rest = D > R && ((Hq && q != q_out) || (Hk && k != k_out));
+  const int v = dtype == OC_DT_F32 ? 4 : 8;
+  bool vec = D % (2 * v) == 0 && R % (2 * v) == 0;
+  for (const oc::RopeTensor& t : p.t)
+    if (t.H && (!aligned(t.x, 16) || !aligned(t.y, 16) || t.xst % v || t.xsh % v || t.yst % v || t.ysh % v)) vec = false;
+  // without vectors the copied part moves in units of two values
+  if (!vec && p.copy_rest && (D - R) % 2 != 0)
+    return fail(OC_ERR_INVALID, "rope: D=%d must be even out of place", D);
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  const int sms = sm_count(dev);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (dtype == OC_DT_F16) return launch_rope_dt<oc::kF16, 8>(p, vec, interleaved != 0, sms, stream);
+  if (dtype == OC_DT_BF16) return launch_rope_dt<oc::kBF16, 8>(p, vec, interleaved != 0, sms, stream);
+  return launch_rope_dt<oc::kF32, 4>(p, vec, interleaved != 0, sms, stream);
+}
+
+extern "C" size_t oc_b200_attention_workspace(int D) {
+  if (D <= 0 || D > 256) return 0;
+  int dev = 0;
+  if (current_device(&dev)) return 0;
+  const int dp = attn_dp(D);
+  return split_ws_bytes(dp, split_ctas(dp, sm_count(dev)));
+}
+
+extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                                 const void* v, int64_t v_st, int64_t v_sh, void* out, int64_t o_st, int64_t o_sh,
+                                 int dtype, int Tq, int Tk, int Hq, int Hkv, int D, const int32_t* cu_q,
+                                 const int32_t* cu_k, const int32_t* kv_lens, int B, int causal, float scale,
+                                 int max_q, int zero_tail, void* workspace, size_t workspace_bytes,
+                                 oc_stream_t stream_) {
+  if (!dt16(dtype)) return fail(OC_ERR_INVALID, "attention: dtype %d (f16 or bf16)", dtype);
+  if (Tq < 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
+    return fail(OC_ERR_INVALID, "attention: Tq=%d Tk=%d B=%d Hq=%d Hkv=%d (Hq a multiple of Hkv)", Tq, Tk, B, Hq, Hkv);
+  if (D <= 0 || D > 256 || D % 8 != 0)
+    return fail(OC_ERR_UNSUPPORTED, "attention: head size %d (a multiple of 8 up to 256)", D);
+  if ((cu_q == nullptr) != (cu_k == nullptr)) return fail(OC_ERR_INVALID, "attention: cu_q and cu_k come together");
+  if (!cu_q && B != 1) return fail(OC_ERR_INVALID, "attention: B=%d without sequence tables", B);
+  if (!std::isfinite(scale)) return fail(OC_ERR_INVALID, "attention: scale %g", (double)scale);
+  if (Tq == 0 || (B == 0 && !zero_tail)) return OC_OK;
+  if (!q || !out || (Tk > 0 && (!k || !v))) return fail(OC_ERR_INVALID, "attention: NULL pointer");
+  const void* ptrs[4] = {q, Tk > 0 ? k : q, Tk > 0 ? v : q, out};
+  const int64_t strides[8] = {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh};
+  for (const void* ptr : ptrs)
+    if (!aligned(ptr, 16)) return fail(OC_ERR_INVALID, "attention: tensors must be 16-byte aligned");
+  for (int64_t st : strides)
+    if (st % 8 != 0 || st < 0)
+      return fail(OC_ERR_INVALID, "attention: stride %lld (a multiple of 8 elements)", (long long)st);
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  const int dp = attn_dp(D);
+  const int ctas = split_ctas(dp, sm_count(dev));
+  oc::AttnParams p{};
+  p.q = reinterpret_cast<const uint16_t*>(q);
+  p.k = reinterpret_cast<const uint16_t*>(Tk > 0 ? k : q);
+  p.v = reinterpret_cast<const uint16_t*>(Tk > 0 ? v : q);
+  p.out = reinterpret_cast<uint16_t*>(out);
+  p.q_st = q_st; p.q_sh = q_sh; p.k_st = k_st; p.k_sh = k_sh;
+  p.v_st = v_st; p.v_sh = v_sh; p.o_st = o_st; p.o_sh = o_sh;
+  p.Tq = Tq; p.Tk = Tk; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.D = D;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.kv_lens = kv_lens;
+  p.B = B;
+  p.causal = causal != 0;
+  p.zero_tail = zero_tail != 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  (void)max_q;
+  if (!workspace || workspace_bytes < split_ws_bytes(dp, ctas) || !aligned(workspace, 16))
+    return fail(OC_ERR_WORKSPACE, "attention: needs %zu bytes of 16-byte aligned workspace, got %zu",
+                split_ws_bytes(dp, ctas), workspace_bytes);
+  p.desc = reinterpret_cast<int*>(workspace);
+  p.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + split_desc_bytes(ctas));
+  const bool bf16 = dtype == OC_DT_BF16;
+  if (dp == 64) return bf16 ? launch_split<true, 64>(p, ctas, stream) : launch_split<false, 64>(p, ctas, stream);
+  if (dp == 128) return bf16 ? launch_split<true, 128>(p, ctas, stream) : launch_split<false, 128>(p, ctas, stream);
+  return bf16 ? launch_split<true, 256>(p, ctas, stream) : launch_split<false, 256>(p, ctas, stream);
+}
+
+extern "C" int oc_b200_dense_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int M, int N,
+                                  int K, const void* bias, int bias_dtype, const void* residual, int64_t ldr, int act,
+                                  void* c, int64_t ldc, oc_stream_t stream_) {
+  if (!dt16(dtype)) return fail(OC_ERR_INVALID, "dense_gemm: dtype %d (f16 or bf16)", dtype);
+  if (M < 0 || N < 0 || K <= 0 || K % 8 != 0)
+    return fail(OC_ERR_INVALID, "dense_gemm: M=%d N=%d K=%d (K a multiple of 8)", M, N, K);
+  if (act < OC_ACT_NONE || act > OC_ACT_RELU) return fail(OC_ERR_INVALID, "dense_gemm: act %d", act);
+  if (bias && !dtf(bias_dtype)) return fail(OC_ERR_INVALID, "dense_gemm: bias dtype %d", bias_dtype);
+  if (M == 0 || N == 0) return OC_OK;
+  if (!x || !w || !c) return fail(OC_ERR_INVALID, "dense_gemm: NULL pointer");
+  if (!aligned(x, 16) || !aligned(w, 16) || ldx % 8 != 0 || ldw % 8 != 0 || ldx < K || ldw < K)
+    return fail(OC_ERR_INVALID, "dense_gemm: X and W rows must be 16-byte aligned (ldx=%lld ldw=%lld)", (long long)ldx,
+                (long long)ldw);
+  if (ldc < N || (residual && ldr < N))
+    return fail(OC_ERR_INVALID, "dense_gemm: ldc=%lld ldr=%lld for N=%d", (long long)ldc, (long long)ldr, N);
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  oc::DenseParams p{};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.bias = bias;
+  p.bias_dtype = bias_dtype;
+  p.residual = reinterpret_cast<const uint16_t*>(residual);
+  p.ldr = ldr;
+  p.act = act;
+  p.out = reinterpret_cast<uint16_t*>(c);
+  p.ldc = ldc;
+  p.vec = aligned(c, 16) && ldc % 8 == 0 && (!residual || (aligned(residual, 16) && ldr % 8 == 0));
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  return dtype == OC_DT_BF16 ? launch_dense<true>(x, ldx, w, ldw, p, dev, stream)
+                             : launch_dense<false>(x, ldx, w, ldw, p, dev, stream);
+}

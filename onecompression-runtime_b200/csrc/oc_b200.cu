@@ -1,5 +1,5 @@
 // C ABI of the onecomp B200 hot path: argument checks, launch configuration,
-// TMA descriptors and kernel dispatch. One translation unit (no -rdc).
+// TMA descriptors and kernel dispatch (block_ops.cu holds the block operators; no -rdc).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -13,6 +13,7 @@
 
 #include "../../include/oc_b200.h"
 #include "common.cuh"
+#include "host.h"
 #include "dequant.cuh"
 #include "gemm_rows.cuh"
 #include "gemm_tc.cuh"
@@ -24,30 +25,9 @@
 #include "allreduce.cuh"
 #include "moe.cuh"
 
+int block_ops_device_error(unsigned* value, cudaStream_t stream);   // block_ops.cu's error word
+
 namespace {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-int cuda_check(cudaError_t e, const char* what) {
-  if (e == cudaSuccess) return OC_OK;
-  return fail(OC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-int launch_check(const char* what) { return cuda_check(cudaGetLastError(), what); }
-
-bool dt16(int dt) { return dt == OC_DT_F16 || dt == OC_DT_BF16; }
-bool dtf(int dt) { return dt == OC_DT_F16 || dt == OC_DT_BF16 || dt == OC_DT_F32; }
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 std::atomic<int> g_opt_path{0}, g_opt_tile{0}, g_opt_gemv_ctas{2}, g_opt_gemv_impl{4}, g_opt_tc_pair{1};
 // failure tests only: bound of the decode GEMV's pipeline waits (0: OC_WAIT_NS) and the stage its
@@ -58,95 +38,19 @@ std::atomic<int> g_opt_wait_us{0}, g_opt_test_stall{0};
 std::atomic<int> g_opt_tc_max_ctas{0};
 std::atomic<int> g_opt_gemv_prep{1};
 
-constexpr int kMaxDevices = 64;
 // Tickets at the head of every GEMV workspace, zero between launches (each launch re-arms the ones it
 // takes): one per 128-column tile for the split-K kernels (at most 256 tiles), one per (256-column
 // tile, consumer warp) for the stream-K kernel (at most 256 tiles x 8 warps).
 constexpr size_t kTicketBytes = 8192;
 constexpr int kSplitTilesMax = 256;
 constexpr int kSkTilesMax = (int)(kTicketBytes / 4) / oc::kSkWarps;
-int g_sm_count[kMaxDevices];
 std::mutex g_mu;
-
-int current_device(int* dev) { return cuda_check(cudaGetDevice(dev), "cudaGetDevice"); }
-
-int sm_count(int dev) {
-  if (dev < 0 || dev >= kMaxDevices) return 148;
-  if (g_sm_count[dev] == 0) {
-    int v = 0;
-    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-    g_sm_count[dev] = v > 0 ? v : 148;
-  }
-  return g_sm_count[dev];
-}
 
 // CTAs of a persistent tcgen05 GEMM: one per SM, or fewer under OC_OPT_TC_MAX_CTAS.
 int tc_ctas(int dev) {
   const int sms = sm_count(dev);
   const int cap = g_opt_tc_max_ctas.load();
   return (cap > 0 && cap < sms) ? cap : sms;
-}
-
-// Launch with programmatic stream serialization (PDL): the kernel may start while the previous
-// kernel in the stream finishes, and orders itself with griddepcontrol.wait.
-template <typename... KArgs, typename... Args>
-int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char* what,
-               Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (int rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...), what)) return rc;
-  return launch_check(what);
-}
-
-int grid_1d(long long total, int threads, int dev) {
-  long long blocks = (total + threads - 1) / threads;
-  long long cap = (long long)sm_count(dev) * 16;
-  if (blocks > cap) blocks = cap;
-  return (int)(blocks < 1 ? 1 : blocks);
-}
-
-// ---- cuTensorMapEncodeTiled through the runtime's driver entry point -------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, int esize, const void* base, uint64_t inner,
-                 uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
-                 CUtensorMapSwizzle swz) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return fail(OC_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
-  if (!aligned(base, 16) || row_stride_bytes % 16 != 0 || (box_inner * esize) % 16 != 0)
-    return fail(OC_ERR_INVALID, "TMA operand alignment: base %p stride %llu", base,
-                (unsigned long long)row_stride_bytes);
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_stride_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(OC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return OC_OK;
 }
 
 }  // namespace
@@ -255,16 +159,18 @@ int oc_b200_get_option(int key, int* value) {
 
 int oc_b200_read_device_error(int* code, oc_stream_t stream) {
   if (!code) return fail(OC_ERR_INVALID, "code is NULL");
-  unsigned v = 0, zero = 0;
+  unsigned v = 0, zero = 0, v_block = 0;
   int rc = cuda_check(cudaMemcpyFromSymbolAsync(&v, oc::g_oc_dev_error, sizeof(v), 0, cudaMemcpyDeviceToHost, stream),
                       "read device error");
   if (rc) return rc;
   rc = cuda_check(cudaMemcpyToSymbolAsync(oc::g_oc_dev_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream),
                   "clear device error");
   if (rc) return rc;
+  rc = block_ops_device_error(&v_block, stream);
+  if (rc) return rc;
   rc = cuda_check(cudaStreamSynchronize(stream), "sync");
   if (rc) return rc;
-  *code = (int)v;
+  *code = (int)(v ? v : v_block);
   return OC_OK;
 }
 

@@ -15,6 +15,7 @@ from . import backend, quant_utils
 from .diffusion import load_int4_model
 from .layers import (
     Dsv4PackedLinear,
+    EagerLinear,
     FusedInt4Linear,
     FusedInt4LinearAnyGroup,
     FusedInt4LinearPaddedGroups,
@@ -24,9 +25,12 @@ from .layers import (
     PackedInt4Conv1d,
     PackedInt4ConvTranspose1d,
     PackedRTNLinear,
+    RotaryEmbedding,
     dequant_dsv4_packed,
     fused_int4_gemm,
     gemlite_available,
+    linear_fused,
+    packed_attention,
     replace_conv_with_packed,
 )
 
@@ -48,6 +52,10 @@ __all__ = [
     "PackedEmbedding",
     "Dsv4PackedLinear",
     "dequant_dsv4_packed",
+    "EagerLinear",
+    "linear_fused",
+    "packed_attention",
+    "RotaryEmbedding",
     "backend",
     "quant_utils",
 ]

@@ -30,6 +30,7 @@ import torch
 from . import _lib
 from .layers.fused_int4_linear import FusedInt4Linear, FusedInt4LinearAnyGroup, FusedInt4LinearPaddedGroups
 from .layers import gemlite_available
+from .layers.dense_linear import EagerLinear
 from .layers.packed_gptq_linear import PackedGPTQLinear
 from .quant_utils import dequant_gptq_to_fp
 
@@ -172,7 +173,7 @@ def build_eager(entry: dict, st: dict, dtype: torch.dtype, device: torch.device)
         wbits=int(entry.get("wbits", 4)),
     )
     has_bias = "bias" in st
-    lin = torch.nn.Linear(in_f, out_f, bias=has_bias, device=device, dtype=dtype)
+    lin = EagerLinear(in_f, out_f, bias=has_bias, device=device, dtype=dtype)
     with torch.no_grad():
         lin.weight.copy_(weight)
         if has_bias:

@@ -6,6 +6,8 @@
 - :class:`PackedGPTQLinear` -- 4/8-bit, any groupsize, act-order, v1/v2;
 - :class:`PackedRTNLinear` / :class:`PackedEmbedding` -- RTN uint8-nibble layers;
 - :class:`Dsv4PackedLinear` / :func:`dequant_dsv4_packed` -- int4/int2 byte-packed layers;
+- :class:`RotaryEmbedding`, :func:`packed_attention`, :func:`linear_fused` / :class:`EagerLinear` --
+  what a transformer block needs between and beside the packed layers (no reference counterpart);
 - :class:`PackedInt4Conv1d` / :class:`PackedInt4ConvTranspose1d` and the conv codec helpers.
 
 GemLite is not part of this build: ``GemLiteInt4Linear`` imports but raises on construction
@@ -13,6 +15,8 @@ and ``gemlite_available()`` reports whether GemLite is importable.
 """
 from __future__ import annotations
 
+from .attention import packed_attention
+from .dense_linear import EagerLinear, linear_fused
 from .dsv4_packed_linear import Dsv4PackedLinear, dequant_dsv4_packed
 from .fused_int4_linear import (
     FusedInt4Linear,
@@ -30,6 +34,7 @@ from .packed_conv import (
 )
 from .packed_gptq_linear import PackedGPTQLinear
 from .packed_linear import PackedEmbedding, PackedRTNLinear
+from .rotary import RotaryEmbedding, rotary_frequencies
 
 
 __all__ = [
@@ -49,4 +54,9 @@ __all__ = [
     "PackedEmbedding",
     "Dsv4PackedLinear",
     "dequant_dsv4_packed",
+    "EagerLinear",
+    "linear_fused",
+    "packed_attention",
+    "RotaryEmbedding",
+    "rotary_frequencies",
 ]

@@ -1,0 +1,45 @@
+"""Argument checks shared by the transformer-block operators (rotary positions, attention, dense linear)."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from .. import _lib
+
+
+def inference_only(what: str, *tensors: torch.Tensor | None) -> None:
+    """The operators have no backward pass: refuse inputs that autograd would track."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference only (no backward pass): call it under torch.no_grad() or detach "
+                           "the inputs")
+
+
+def one_device(what: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
+    """The B200 device all tensors live on."""
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    _lib.require_b200(first.device)
+    return first.device
+
+
+def on_device(dev: torch.device):
+    """Make ``dev`` current for the launch if it is not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte and one past the last byte that the tensor's elements touch."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
+    """Whether the address ranges of two tensors meet (interleaved column slices of one buffer do)."""
+    if b is None:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
