@@ -7,12 +7,23 @@ of the video-DiT stack, the 5120-wide decode layers; wide heads rotated in part 
 """
 import math
 import random
+import sys
+from pathlib import Path
 
 import torch
 
 own = False
 
 _DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _layers():
+    """The framework's layers; the package lies one folder below the repository's root."""
+    root = str(Path(__file__).resolve().parents[1] / "onecompression-runtime_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from onecomp_runtime import layers
+    return layers
 
 
 # ------------------------------------------------------------------------------------------- cases
@@ -152,9 +163,8 @@ def prepare(case, seed):
                   k=qkv[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d)),
                   pos=torch.randint(0, case["far"], shape, generator=g, device=dev, dtype=torch.int64))
         if own:
-            from onecomp_runtime.layers import RotaryEmbedding
-            st["rope"] = RotaryEmbedding(d, rotary_dim=case["rot"], layout=case["layout"], axes=axes,
-                                         scaling=_rope_scaling(case), device=dev)
+            st["rope"] = _layers().RotaryEmbedding(d, rotary_dim=case["rot"], layout=case["layout"], axes=axes,
+                                                   scaling=_rope_scaling(case), device=dev)
         else:
             freq, gain = _frequencies(case, axes)
             st["freq"], st["gain"] = torch.tensor(freq, dtype=torch.float64, device=dev), gain
@@ -186,7 +196,7 @@ def run(state):
 
 
 def _run_own(op, st):
-    from onecomp_runtime import layers
+    layers = _layers()
     if op in ("decode", "prompt"):
         return layers.packed_attention(st["q"], st["k"], st["v"], st["cu_q"], st["cu_k"], kv_lens=st.get("kv_lens"),
                                        causal=st["case"].get("causal", True), max_seqlen_q=st["max_q"])
