@@ -1,0 +1,451 @@
+// Attention for prompts: many query rows per sequence, on the 5th-generation tensor cores.
+//
+// Bound by the tensor pipe and, at head size 64 and 128, by the exponentials (16 a cycle and SM against
+// 8192 tensor operations). One CTA per 128-row tile pair of one query head (one tile where the head
+// size is 256): S = Q K^T and O += P V as tcgen05 MMAs of 128 x 128 x 16 into TMEM, one pass over the
+// keys in blocks of 128.
+//   * A softmax warpgroup per tile, one thread per row: it reads S from TMEM (no shuffles), writes the
+//     16-bit weights P back to TMEM as the A operand of the second product, and keeps maximum and sum
+//     in registers. While one tile is in its softmax the tensor pipe runs the other tile's products.
+//   * The reference that the exponents are taken against follows the running maximum only when
+//     it grows by more than 2^8: weights up to 256 are as exact in 16 bits as weights up to 1, and
+//     the accumulator in TMEM is read, scaled and written back only in those rare steps.
+//   * K and V move by TMA in units of [128 keys x 64 columns] (128-byte swizzle) through one ring that
+//     both tiles of the CTA share; V is read by the MMA in its own layout (MN-major B operand).
+//   * Two warps prepare the V blocks at the end of what the rows see (the causal diagonal, the end
+//     of the sequence): rows behind the keys become zeros, and in causal blocks infinities and NaN,
+//     which a weight of zero must not turn into NaN, are taken out and added afterwards by the rows
+//     that see them.
+// Tiles are numbered without the host knowing a length: sequence b's tiles start at
+// floor(cu_q[b] / rows) + b, which leaves room for every sequence's ragged last tile; a CTA whose tile
+// lies behind its sequence's end exits. Every head's tiles run from its last row up, so that the long
+// causal tiles start first. All waits are bounded (common.cuh).
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace oc {
+
+constexpr int kTileKeys = 128;
+constexpr int kTileUnitBytes = 128 * 128;   // [128 rows x 64 columns] of 16-bit values
+constexpr int kTileMaxEdges = 3;
+
+template <int DP> struct TileCfg {
+  static constexpr int kTiles = DP == 256 ? 1 : 2;          // row tiles of a CTA
+  static constexpr int kRows = kTiles * 128;
+  static constexpr int kUnits = DP / 64;                    // units of a K or V block
+  static constexpr int kSlots = DP == 256 ? 2 : DP == 128 ? 5 : 10;
+  static constexpr int kSoftmaxThreads = kTiles * 128;
+  static constexpr int kThreads = kSoftmaxThreads + 128;
+  static constexpr int kQBytes = kTiles * kUnits * kTileUnitBytes;
+  static constexpr int kRingBytes = kSlots * kUnits * kTileUnitBytes;
+  static constexpr int kBars = 2 * kSlots * kUnits + 1 + 2 + 2 + 2 + 2 * kTileMaxEdges + 1;
+  static constexpr int kSmem = kQBytes + kRingBytes + 1024 + kBars * 8 + 32;
+  static constexpr uint32_t kOCol = 256;
+  __device__ static uint32_t s_col(int i) { return i * 128; }
+  // P shares the columns of its S (read by then), except where the head leaves TMEM to spare
+  __device__ static uint32_t p_col(int i) { return DP == 64 ? 384 + i * 64 : i * 128; }
+  __device__ static uint32_t o_col(int t) { return kOCol + t * DP; }
+  static_assert(kSmem <= 232448, "shared memory per CTA");
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// MN-major operand with the 128-byte swizzle: rows of 64 values along N (128 B), 8-row atoms along K
+// 1024 B apart, groups of 64 along N one unit apart.
+__device__ __forceinline__ uint64_t smem_desc_mnmajor_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(kTileUnitBytes >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+struct TileMaps { CUtensorMap q, k, v; };
+
+// What a CTA works on; every role derives the same numbers.
+struct TileWork {
+  Seq s;
+  int head, kvh, r0, ntile, nblk, e0;   // e0: first block that some row of the CTA does not see whole
+  int nb[2];                            // blocks of each tile
+};
+
+template <int DP> __device__ __forceinline__ bool tile_work(const AttnParams& p, int n_slots, TileWork& w) {
+  constexpr int R = TileCfg<DP>::kRows;
+  w.head = blockIdx.x / n_slots;
+  const int slot = n_slots - 1 - blockIdx.x % n_slots;
+  int lo = 0, hi = p.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int q0 = p.cu_q ? min(max(p.cu_q[mid], 0), p.Tq) : 0;
+    if (q0 / R + mid <= slot) lo = mid; else hi = mid;
+  }
+  w.s = attn_seq(p, lo);
+  const long long r0 = (long long)(slot - (w.s.q0 / R + lo)) * R;
+  if (r0 < 0 || r0 >= w.s.nq) return false;
+  w.r0 = (int)r0;
+  w.kvh = w.head / p.G;
+  w.ntile = min(TileCfg<DP>::kTiles, (w.s.nq - w.r0 + 127) / 128);
+  const int off = w.s.nk - w.s.nq;
+  for (int t = 0; t < 2; ++t) {
+    const int last = min(w.s.nq, w.r0 + (t + 1) * 128) - 1;
+    const int keys = p.causal ? min(w.s.nk, max(0, last + off + 1)) : w.s.nk;
+    w.nb[t] = t < w.ntile ? (keys + kTileKeys - 1) / kTileKeys : 0;
+  }
+  w.nblk = w.nb[w.ntile - 1];
+  const int all = p.causal ? max(0, min(w.s.nk, w.r0 + off + 1)) : w.s.nk;   // keys that the first row sees
+  w.e0 = min(all / kTileKeys, w.nblk);
+  return true;
+}
+
+// Sequence number in the ring of block j's K and V loads, in the order the MMAs take them.
+template <int DP> __device__ __forceinline__ int k_use(int j) { return TileCfg<DP>::kTiles == 2 || j == 0 ? 2 * j : 2 * j - 1; }
+template <int DP> __device__ __forceinline__ int v_use(int j, int nblk) {
+  return TileCfg<DP>::kTiles == 2 || j == nblk - 1 ? 2 * j + 1 : 2 * j + 2;
+}
+
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
+    attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const int n_slots, const int negate) {
+  using Cfg = TileCfg<DP>;
+  constexpr int U = Cfg::kUnits, NU = Cfg::kSlots * U;
+  constexpr bool kTwo = Cfg::kTiles == 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* ring = smem + Cfg::kQBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + Cfg::kRingBytes);
+  uint64_t* empty = full + NU;
+  uint64_t* q_full = empty + NU;
+  uint64_t* s_full = q_full + 1;            // [2] by tile, or by block parity where there is one tile
+  uint64_t* p_full = s_full + 2;            // [2]
+  uint64_t* pv_done = p_full + 2;           // [2] by tile
+  uint64_t* edge_full = pv_done + 2;        // [3] V blocks from e0 on: loaded
+  uint64_t* edge_ready = edge_full + kTileMaxEdges;   // [3] and prepared
+  uint64_t* drain = edge_ready + kTileMaxEdges;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile int* odd_values = abort_flag + 1;   // an infinity or NaN was taken out of a V block
+  const int warp = warp_id(), lane = lane_id();
+
+  if (p.zero_tail) attn_zero_tail(p, blockIdx.x, gridDim.x);
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.B; b += Cfg::kThreads) attn_seq(p, b, true);
+  TileWork w;
+  if (!tile_work<DP>(p, n_slots, w)) return;
+  const Seq s = w.s;
+  const int off = s.nk - s.nq;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NU; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1); }
+    for (int i = 0; i < kTileMaxEdges; ++i) { mbar_init(&edge_full[i], 1); mbar_init(&edge_ready[i], 64); }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *odd_values = 0;
+    fence_barrier_init();
+  }
+  constexpr int kAux = Cfg::kSoftmaxThreads / 32;   // first warp of the last warpgroup: TMA, MMA, V, V
+  if (warp == kAux + 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp >= kAux) {
+    if constexpr (kTwo) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kAux) {
+      // ------------------------------------------------------------ TMA
+      if (lane == 0) {
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+        mbar_arrive_expect_tx(q_full, w.ntile * U * kTileUnitBytes);
+        for (int t = 0; t < w.ntile; ++t)
+          for (int u = 0; u < U; ++u)
+            tma_load_3d(q_smem + (t * U + u) * kTileUnitBytes, &maps.q, q_full, u * 64, w.head, s.q0 + w.r0 + t * 128);
+        int edges = 0, uses = 0;
+        bool ok = true;
+        for (int n = 0; ok && n < 2 * w.nblk; ++n) {
+          // the n-th block in the MMAs' order
+          int j = n >> 1;
+          bool is_v = n & 1;
+          if (!kTwo && n > 0 && n < 2 * w.nblk - 1) { is_v = !(n & 1); j = is_v ? (n - 2) >> 1 : (n + 1) >> 1; }
+          const int slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
+          const bool edge = is_v && j >= w.e0;
+          if (edge) {
+            mbar_arrive_expect_tx(&edge_full[j - w.e0], U * kTileUnitBytes);
+            ++edges;
+          }
+          for (int u = 0; u < U; ++u) {
+            const int i = slot * U + u;
+            if (!mbar_wait(&empty[i], par ^ 1, abort_flag, kDevErrTmaEmpty)) {
+              // an edge block was announced: its remaining bytes never come, so nobody drains it
+              if (edge) --edges;
+              ok = false;
+              break;
+            }
+            uint64_t* bar = edge ? &edge_full[j - w.e0] : &full[i];
+            if (edge) mbar_arrive(&full[i]);   // the ring's phases go on; the block is announced on its own barrier
+            else mbar_arrive_expect_tx(&full[i], kTileUnitBytes);
+            tma_load_3d(ring + i * kTileUnitBytes, is_v ? &maps.v : &maps.k, bar, u * 64, w.kvh, s.k0 + j * kTileKeys);
+            ++uses;
+          }
+        }
+        // every load issued lands before the CTA exits (consumed ones return at once)
+        mbar_drain(q_full, 0);
+        for (int i = uses > NU ? uses - NU : 0; i < uses; ++i) mbar_drain(&full[i % NU], (i / NU) & 1);
+        for (int e = 0; e < edges; ++e) mbar_drain(&edge_full[e], 0);
+      }
+    } else if (warp == kAux + 1) {
+      // ------------------------------------------------------------ MMA
+      if (lane == 0) {
+        const uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128) | (negate ? 1u << 13 : 0u);
+        constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, DP) | (1u << 16);   // B is MN-major
+        const int last_tile = w.ntile - 1;
+        auto qk = [&](int t, int j) {
+          const int n = k_use<DP>(j), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
+          const int b = kTwo ? t : (j & 1);
+          for (int u = 0; u < U; ++u) {
+            const int i = slot * U + u;
+            if (!mbar_wait(&full[i], par, abort_flag, kDevErrTmaFull)) return false;
+            tc_fence_after();
+            const uint32_t qa = smem_u32(q_smem + (t * U + u) * kTileUnitBytes), ka = smem_u32(ring + i * kTileUnitBytes);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_ss(tmem + Cfg::s_col(b), smem_desc_kmajor_sw128(qa + k * 32), smem_desc_kmajor_sw128(ka + k * 32),
+                        idesc_qk, (u | k) != 0 ? 1u : 0u);
+            if (t == last_tile) tc_commit(&empty[i]);
+          }
+          tc_commit(&s_full[b]);
+          return true;
+        };
+        auto pv = [&](int t, int j) {
+          const int n = v_use<DP>(j, w.nblk), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
+          const int b = kTwo ? t : (j & 1);
+          if (j >= w.e0) {
+            if (!mbar_wait(&edge_ready[j - w.e0], 0, abort_flag, kDevErrWFull)) return false;
+          } else {
+            for (int u = 0; u < U; ++u)
+              if (!mbar_wait(&full[slot * U + u], par, abort_flag, kDevErrTmaFull)) return false;
+          }
+          if (!mbar_wait(&p_full[b], kTwo ? (j & 1) : ((j >> 1) & 1), abort_flag, kDevErrAFull)) return false;
+          tc_fence_after();
+          const uint32_t va = smem_u32(ring + slot * U * kTileUnitBytes);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(b) + k * 8, smem_desc_mnmajor_sw128(va + k * 2048),
+                      idesc_pv, (j | k) != 0 ? 1u : 0u);
+          if (t == last_tile)
+            for (int u = 0; u < U; ++u) tc_commit(&empty[slot * U + u]);
+          tc_commit(&pv_done[t]);
+          return true;
+        };
+        // S(j + 1) overwrites the columns of P(j) (two tiles) or P(j - 1) (one tile): only once the
+        // product that reads them is done
+        auto pv_over = [&](int t, int j) {
+          return mbar_wait(&pv_done[t], j & 1, abort_flag, kDevErrAccFull);
+        };
+        bool ok = mbar_wait(q_full, 0, abort_flag, kDevErrResFull);
+        if constexpr (kTwo) {
+          for (int t = 0; ok && t < w.ntile; ++t)
+            if (w.nb[t] > 0) ok = qk(t, 0);
+          for (int j = 0; ok && j < w.nblk; ++j)
+            for (int t = 0; ok && t < w.ntile; ++t) {
+              if (j < w.nb[t]) ok = pv(t, j);
+              if (ok && j + 1 < w.nb[t]) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(t, j)) && qk(t, j + 1);
+            }
+        } else {
+          if (w.nblk > 0) ok = ok && qk(0, 0);
+          for (int j = 0; ok && j < w.nblk; ++j) {
+            if (j + 1 < w.nblk) ok = (j == 0 || pv_over(0, j - 1)) && qk(0, j + 1);
+            if (ok) ok = pv(0, j);
+          }
+        }
+        tc_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    } else {
+      // ------------------------------------------------------------ V blocks at the end of what rows see
+      const int tid = threadIdx.x - (kAux + 2) * 32;
+      for (int e = 0; w.e0 + e < w.nblk; ++e) {
+        const int j = w.e0 + e;
+        if (!mbar_wait(&edge_full[e], 0, abort_flag, kDevErrWEmpty)) break;
+        const int n = v_use<DP>(j, w.nblk), slot = n % Cfg::kSlots;
+        uint4* blk = reinterpret_cast<uint4*>(ring + slot * U * kTileUnitBytes);
+        bool odd = false;
+        if (p.causal || j * kTileKeys + kTileKeys > s.nk) {
+#pragma unroll 4
+          for (int i = tid; i < U * 1024; i += 64) {
+            const int key = j * kTileKeys + ((i & 1023) >> 3);   // the swizzle moves 16-byte chunks inside a row only
+            if (key >= s.nk) {
+              blk[i] = make_uint4(0, 0, 0, 0);
+            } else if (p.causal) {
+              uint4 x = blk[i];
+              if (nonfinite2<BF16>(x.x) || nonfinite2<BF16>(x.y) || nonfinite2<BF16>(x.z) || nonfinite2<BF16>(x.w)) {
+                x.x = finite2<BF16>(x.x); x.y = finite2<BF16>(x.y); x.z = finite2<BF16>(x.z); x.w = finite2<BF16>(x.w);
+                blk[i] = x;
+                odd = true;
+              }
+            }
+          }
+        }
+        if (odd) *odd_values = 1;
+        fence_proxy_async_shared();
+        mbar_arrive(&edge_ready[e]);
+      }
+    }
+  } else {
+    // -------------------------------------------------------------- softmax: one thread per row
+    if constexpr (kTwo) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int row = w.r0 + t * 128 + (warp & 3) * 32 + lane;
+    const int limit = p.causal ? min(s.nk - 1, row + off) : s.nk - 1;                  // last key this row sees
+    const int limit0 = p.causal ? min(s.nk - 1, row - lane + off) : s.nk - 1;          // of the warp's first row
+    const float sc = p.scale_log2;
+    const float grow = 8.f / sc;
+    float m = -INFINITY, l = 0.f;
+    bool ok = t < w.ntile;
+    const int nb = w.nb[t];
+    for (int j = 0; ok && j < nb; ++j) {
+      const int b = kTwo ? t : (j & 1);
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], kTwo ? (j & 1) : ((j >> 1) & 1), abort_flag, kDevErrAccFull));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tmem + lanes + Cfg::s_col(b) + c * 32, v[c]);
+      tc_wait_ld();
+      if (j * kTileKeys + kTileKeys - 1 > limit0) {
+        const int seen = limit - j * kTileKeys;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i > seen) v[c][i] = 0xff800000u;
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+      }
+      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+      if (j == 0) {
+        m = top;
+      } else {
+        const bool need = top - m > grow;
+        if (__any_sync(0xffffffffu, need)) {
+          // scale what is accumulated; the product that adds to it is done first
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (j - 1) & 1, abort_flag, kDevErrAccEmpty));
+          if (!ok) break;
+          tc_fence_after();
+          const float f = need ? ex2((m - top) * sc) : 1.f;
+          if (need) m = top;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tmem + lanes + Cfg::o_col(t) + c * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_32x32b_x32(tmem + lanes + Cfg::o_col(t) + c * 32, o);
+          }
+        }
+      }
+      const float bias = m == -INFINITY ? 0.f : -m * sc;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p0 = ex2(fmaf(__uint_as_float(v[c][2 * i]), sc, bias));
+          const float p1 = ex2(fmaf(__uint_as_float(v[c][2 * i + 1]), sc, bias));
+          sum[0] += p0;
+          sum[1] += p1;
+          pk[i] = pack2_rn<BF16>(p0, p1);
+        }
+        tmem_st_32x32b_x16(tmem + lanes + Cfg::p_col(b) + c * 16, pk);
+      }
+      l += sum[0] + sum[1];
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[b]);
+    }
+    // the row's output
+    if (ok && nb > 0) ok = mbar_wait(&pv_done[t], (nb - 1) & 1, abort_flag, kDevErrAccEmpty);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      uint16_t* dst = p.out + (long long)(s.q0 + row) * p.o_st + w.head * p.o_sh;
+      const bool odd = *odd_values != 0;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        if (nb > 0) {
+          tmem_ld_32x32b_x32(tmem + lanes + Cfg::o_col(t) + c * 32, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (row < s.nq) {
+          if (odd) {   // add the values that were taken out, where this row sees them
+            for (int key = w.e0 * kTileKeys; key <= limit; ++key) {
+              const uint16_t* vr = p.v + (long long)(s.k0 + key) * p.v_st + w.kvh * p.v_sh + c * 32;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i < p.D && nonfinite2<BF16>(vr[i]))
+                  o[i] = __float_as_uint(__uint_as_float(o[i]) + bits_to_f32(vr[i], BF16 ? kBF16 : kF16));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c * 32 + i * 8 < p.D) {
+              uint4 x;
+              x.x = pack2_rn<BF16>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+              x.y = pack2_rn<BF16>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+              x.z = pack2_rn<BF16>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+              x.w = pack2_rn<BF16>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = x;
+            }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kAux + 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace oc

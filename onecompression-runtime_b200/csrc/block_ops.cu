@@ -1,5 +1,6 @@
 // C ABI of the operators between and beside the packed linears of a transformer block: rotary
 // positions, attention over packed sequences, the dense 16-bit linear.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -9,6 +10,10 @@
 #include "rope.cuh"
 #include "attn_common.cuh"
 #include "attn_split.cuh"
+#ifndef OC_ATTN_IN_ORDER
+#define OC_ATTN_IN_ORDER 0
+#endif
+#include "attn_tile.cuh"
 #include "gemm_dense.cuh"
 
 // This translation unit's device error word (common.cuh defines one per unit), for
@@ -58,6 +63,7 @@ int launch_rope_dt(const oc::RopeParams& p, bool vec, bool inter, int sms, cudaS
 }
 
 // ------------------------------------------------------------------ attention
+constexpr int kTileMinRows = 16;
 int attn_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 template <int DP> int split_ctas(int sms) { return sms * oc::SplitCfg<DP>::kCtasPerSm; }
@@ -76,6 +82,40 @@ template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas,
   if (int rc = launch_check("attention (split)")) return rc;
   return launch_pdl(oc::attn_join_kernel<BF16, DP>, dim3((unsigned)ctas, oc::kSplitRows / 4), dim3(128), 0, stream,
                     "attention (join)", p);
+}
+
+// [rows, heads, D] tensor in boxes of 128 rows x one head x 64 columns. A dimension of one row or head
+// takes any valid stride.
+int attn_tmap(CUtensorMap* map, bool bf16, const void* base, int D, int H, int T, int64_t sh, int64_t st) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(OC_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)(H > 1 ? sh : D) * 2, (cuuint64_t)(T > 1 ? st : D) * 2};
+  cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(OC_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return OC_OK;
+}
+
+template <bool BF16, int DP> int launch_tile(oc::AttnParams p, cudaStream_t stream) {
+  using Cfg = oc::TileCfg<DP>;
+  oc::TileMaps maps;
+  if (int rc = attn_tmap(&maps.q, BF16, p.q, p.D, p.Hq, p.Tq, p.q_sh, p.q_st)) return rc;
+  if (int rc = attn_tmap(&maps.k, BF16, p.k, p.D, p.Hkv, p.Tk, p.k_sh, p.k_st)) return rc;
+  if (int rc = attn_tmap(&maps.v, BF16, p.v, p.D, p.Hkv, p.Tk, p.v_sh, p.v_st)) return rc;
+  const int slots = p.Tq / Cfg::kRows + p.B;
+  if ((long long)slots * p.Hq > INT_MAX) return fail(OC_ERR_INVALID, "attention: %d tiles x %d heads", slots, p.Hq);
+  // the softmax takes its maximum before the scale: a negative scale negates Q in the product, and
+  // zero becomes a scale that rounds every finite score to zero but leaves masked ones infinite
+  const int negate = p.scale_log2 < 0.f;
+  p.scale_log2 = std::fmax(std::fabs(p.scale_log2), 1e-30f);
+  auto kern = oc::attn_tile_kernel<BF16, DP>;
+  if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
+  kern<<<slots * p.Hq, Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, slots, negate);
+  return launch_check("attention (tile)");
 }
 
 // ------------------------------------------------------------------ dense linear
@@ -214,13 +254,19 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   p.zero_tail = zero_tail != 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  (void)max_q;
+  const bool bf16 = dtype == OC_DT_BF16;
+  // Query rows of a sequence, as far as the host knows them.
+  const int64_t run = max_q > 0 ? std::min(max_q, Tq) : ((int64_t)Tq + std::max(B, 1) - 1) / std::max(B, 1);
+  if (run > kTileMinRows && B > 0 && Tk > 0) {
+    if (dp == 64) return bf16 ? launch_tile<true, 64>(p, stream) : launch_tile<false, 64>(p, stream);
+    if (dp == 128) return bf16 ? launch_tile<true, 128>(p, stream) : launch_tile<false, 128>(p, stream);
+    return bf16 ? launch_tile<true, 256>(p, stream) : launch_tile<false, 256>(p, stream);
+  }
   if (!workspace || workspace_bytes < split_ws_bytes(dp, ctas) || !aligned(workspace, 16))
     return fail(OC_ERR_WORKSPACE, "attention: needs %zu bytes of 16-byte aligned workspace, got %zu",
                 split_ws_bytes(dp, ctas), workspace_bytes);
   p.desc = reinterpret_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + split_desc_bytes(ctas));
-  const bool bf16 = dtype == OC_DT_BF16;
   if (dp == 64) return bf16 ? launch_split<true, 64>(p, ctas, stream) : launch_split<false, 64>(p, ctas, stream);
   if (dp == 128) return bf16 ? launch_split<true, 128>(p, ctas, stream) : launch_split<false, 128>(p, ctas, stream);
   return bf16 ? launch_split<true, 256>(p, ctas, stream) : launch_split<false, 256>(p, ctas, stream);

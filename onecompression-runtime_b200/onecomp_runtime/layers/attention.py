@@ -20,7 +20,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [tokens, heads, D] if the kernels can address it (unit stride inside a head, 16-byte aligned
     rows), else a contiguous copy."""
     ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0
-    ok = ok and all(n <= 1 or s % 8 == 0 for n, s in zip(t.shape[:2], t.stride()[:2]))
+    ok = ok and all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2]))
     if not ok:
         t = t.contiguous()
         if t.data_ptr() % 16:
@@ -42,8 +42,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     ``q`` [Tq, Hq, D]; ``k``, ``v`` [Tk, Hkv, D], fp16 or bf16, Hq a multiple of Hkv (query head h reads key
     head ``h // (Hq // Hkv)``), D a multiple of 8 up to 256. Any token and head strides, so the column slices
-    of one qkv projection go in as they are (a last dimension that is not contiguous, or rows off 16-byte
-    boundaries, are copied).
+    of one qkv projection go in as they are (a last dimension that is not contiguous, rows off 16-byte
+    boundaries and expanded dimensions are copied).
 
     ``cu_seqlens_q`` / ``cu_seqlens_k``: int32 [B + 1] on the device, first row of each sequence (given
     together; without them all rows are one sequence). ``kv_lens``: int32 [B], how many keys from
