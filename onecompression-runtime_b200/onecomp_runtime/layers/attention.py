@@ -16,22 +16,25 @@ def _workspace_bytes(device_index: int, head_dim: int) -> int:
         return _lib.lib().oc_b200_attention_workspace(head_dim)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [tokens, heads, D] if the kernels can address it (unit stride inside a head, 16-byte aligned
-    rows), else a contiguous copy."""
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0
-    ok = ok and all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2]))
-    if not ok:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
-
-
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    """Token and head strides; a dimension of one row gets the contiguous one (its own may be anything)."""
-    head = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]), head
+def _rows(t: torch.Tensor, copy: bool = True) -> tuple[torch.Tensor, int, int, int] | None:
+    """``t`` [tokens, heads, D] as the kernels address it: (tensor, pointer, token stride, head stride). A
+    layout they cannot address (they need a unit stride inside a head and 16-byte aligned rows) is copied,
+    or gives None. A dimension of one row gets the contiguous stride (its own may be anything)."""
+    st, sh, sd = t.stride()
+    T, H, D = t.shape
+    if H <= 1:
+        sh = D
+    if T <= 1:
+        st = H * D
+    ptr = t.data_ptr()
+    if sd == 1 and ptr % 16 == 0 and st > 0 and sh > 0 and st % 8 == 0 and sh % 8 == 0:
+        return t, ptr, st, sh
+    if not copy:
+        return None
+    t = t.contiguous()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return t, t.data_ptr(), H * D, D
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
@@ -65,45 +68,51 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
     Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[:2]
+    Tk, Hkv, _ = k.shape
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} key heads")
     if D == 0 or D % 8 or D > 256:
         raise ValueError(f"{what}: head size {D} (a multiple of 8 up to 256)")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"{what} takes fp16 or bf16 of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    dtype = q.dtype
+    if dtype not in (torch.float16, torch.bfloat16) or k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{what} takes fp16 or bf16 of one dtype, got {dtype}, {k.dtype}, {v.dtype}")
     if (cu_seqlens_q is None) != (cu_seqlens_k is None):
         raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k come together")
-    tables = (cu_seqlens_q, cu_seqlens_k, kv_lens)
     B = 1 if cu_seqlens_q is None else cu_seqlens_q.numel() - 1
-    for name, t, n in zip(("cu_seqlens_q", "cu_seqlens_k", "kv_lens"), tables, (B + 1, B + 1, B)):
+    for name, t, n in (("cu_seqlens_q", cu_seqlens_q, B + 1), ("cu_seqlens_k", cu_seqlens_k, B + 1),
+                       ("kv_lens", kv_lens, B)):
         if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or n < 1):
             raise ValueError(f"{what}: {name} must be int32 [{max(n, 1)}], got {t.dtype} {tuple(t.shape)}")
     if scale is None:
         scale = D ** -0.5
     if not math.isfinite(scale):
         raise ValueError(f"{what}: scale {scale}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
-        raise ValueError(f"{what}: out is {out.dtype} {tuple(out.shape)}, expected {q.dtype} {tuple(q.shape)}")
+    if out is not None and (out.shape != q.shape or out.dtype != dtype):
+        raise ValueError(f"{what}: out is {out.dtype} {tuple(out.shape)}, expected {dtype} {tuple(q.shape)}")
     inference_only(what, q, k, v, out)
-    dev = one_device(what, q, k, v, out, *tables)
+    dev = one_device(what, q, k, v, out, cu_seqlens_q, cu_seqlens_k, kv_lens)
     if out is not None:
-        if any(overlap(out, t) for t in (q, k, v)):
+        if overlap(out, q) or overlap(out, k) or overlap(out, v):
             raise ValueError(f"{what}: out shares memory with an input")
-        if Tq and _rows(out) is not out:
+        rows_out = _rows(out, copy=False)
+        if rows_out is None:
             raise ValueError(f"{what}: out needs a unit last stride and 16-byte aligned rows")
-        target = out
+        target, o_ptr, o_st, o_sh = rows_out
     else:
-        target = torch.empty((Tq, Hq, D), dtype=q.dtype, device=dev)
+        target = torch.empty((Tq, Hq, D), dtype=dtype, device=dev)
+        o_ptr, o_st, o_sh = target.data_ptr(), Hq * D, D
     if Tq == 0:
         return target
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    cu_q, cu_k, lens = (None if t is None else t.contiguous() for t in tables)
+    q, q_ptr, q_st, q_sh = _rows(q)
+    k, k_ptr, k_st, k_sh = _rows(k)
+    v, v_ptr, v_st, v_sh = _rows(v)
+    cu_q = None if cu_seqlens_q is None else cu_seqlens_q.contiguous()
+    cu_k = None if cu_seqlens_k is None else cu_seqlens_k.contiguous()
+    lens = None if kv_lens is None else kv_lens.contiguous()
     with on_device(dev):
         ws = torch.empty(_workspace_bytes(dev.index, D), dtype=torch.uint8, device=dev)
-        _lib.call("oc_b200_attention", q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
-                  *_strides(v), target.data_ptr(), *_strides(target), _lib.DT[q.dtype], Tq, Tk, Hq, Hkv, D,
-                  _lib.ptr(cu_q), _lib.ptr(cu_k), _lib.ptr(lens), B, int(causal), float(scale),
-                  0 if max_seqlen_q is None else max(0, int(max_seqlen_q)), int(out is None), ws.data_ptr(),
-                  ws.numel(), _lib.stream_of(dev))
+        _lib.call("oc_b200_attention", q_ptr, q_st, q_sh, k_ptr, k_st, k_sh, v_ptr, v_st, v_sh, o_ptr, o_st, o_sh,
+                  _lib.DT[dtype], Tq, Tk, Hq, Hkv, D, _lib.ptr(cu_q), _lib.ptr(cu_k), _lib.ptr(lens), B, causal, scale,
+                  0 if max_seqlen_q is None else max(0, max_seqlen_q), out is None, ws.data_ptr(), ws.numel(),
+                  _lib.stream_of(dev))
     return target

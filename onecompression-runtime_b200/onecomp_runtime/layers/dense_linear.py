@@ -14,7 +14,7 @@ ACTIVATIONS = {None: 0, "none": 0, "gelu_tanh": 1, "gelu": 2, "silu": 3, "relu":
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Rows the TMA can read (unit column stride, 16-byte aligned rows), or a contiguous copy."""
     rows = t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])
-    if t.stride(1) != 1 or t.data_ptr() % 16 or not rows:
+    if not rows or t.stride(1) != 1 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -23,6 +23,25 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _output(what: str, out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+            residual: torch.Tensor | None, M: int, N: int) -> tuple[int, int]:
+    """Pointer and row stride of a given output."""
+    try:
+        rows = out.view(M, N)
+    except RuntimeError as e:
+        raise ValueError(f"{what}: out's leading dimensions must fold into one stride, got {out.stride()}") from e
+    if rows.numel() and N > 1 and rows.stride(1) != 1:
+        raise ValueError(f"{what}: out needs a unit column stride, got {out.stride()}")
+    if M > 1 and rows.stride(0) < N:
+        raise ValueError(f"{what}: out rows overlap (strides {out.stride()})")
+    if overlap(rows, x) or overlap(rows, weight) or overlap(rows, bias):
+        raise ValueError(f"{what}: out shares memory with an input")
+    if residual is not None and overlap(rows, residual) and \
+            (residual.data_ptr(), _ld(residual), residual.stride(1)) != (rows.data_ptr(), _ld(rows), rows.stride(1)):
+        raise ValueError(f"{what}: out overlaps the residual but is not the residual itself")
+    return rows.data_ptr(), _ld(rows)
 
 
 def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -47,32 +66,21 @@ def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"{what}: activation {activation!r}, one of {sorted(a for a in ACTIVATIONS if a)}")
     if bias is not None and (bias.shape != (N,) or bias.dtype not in _lib.DT):
         raise ValueError(f"{what}: bias {bias.dtype} {tuple(bias.shape)}, expected [{N}] fp16, bf16 or fp32")
-    lead = x.shape[:-1]
+    shape = (*x.shape[:-1], N)
     for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != (*lead, N) or t.dtype != x.dtype):
-            raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, expected {x.dtype} {(*lead, N)}")
+        if t is not None and (t.shape != shape or t.dtype != x.dtype):
+            raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, expected {x.dtype} {shape}")
     inference_only(what, x, weight, bias, residual, out)
     dev = one_device(what, x, weight, bias, residual, out)
-    x2 = x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     M = x2.shape[0]
-    res2 = None if residual is None else residual.reshape(M, N)
+    res2 = residual if residual is None or residual.dim() == 2 else residual.reshape(M, N)
     if out is None:
-        out2 = torch.empty((M, N), dtype=x.dtype, device=dev)
-        target = out2.view(*lead, N)
+        target = torch.empty(shape, dtype=x.dtype, device=dev)
+        o_ptr, ldc = target.data_ptr(), N
     else:
-        try:
-            out2 = out.view(M, N)
-        except RuntimeError as e:
-            raise ValueError(f"{what}: out's leading dimensions must fold into one stride, got {out.stride()}") from e
-        if out2.numel() and out2.stride(1) != 1:
-            raise ValueError(f"{what}: out needs a unit column stride, got {out.stride()}")
-        if M > 1 and out2.stride(0) < N:
-            raise ValueError(f"{what}: out rows overlap (strides {out.stride()})")
-        if overlap(out2, x) or overlap(out2, weight) or overlap(out2, bias):
-            raise ValueError(f"{what}: out shares memory with an input")
-        if res2 is not None and overlap(out2, res2) and (res2.data_ptr(), _ld(res2)) != (out2.data_ptr(), _ld(out2)):
-            raise ValueError(f"{what}: out overlaps the residual but is not the residual itself")
         target = out
+        o_ptr, ldc = _output(what, out, x, weight, bias, res2, M, N)
     if M == 0 or N == 0:
         return target
     x2, w2 = _aligned(x2), _aligned(weight)
@@ -82,7 +90,7 @@ def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     with on_device(dev):
         _lib.call("oc_b200_dense_gemm", x2.data_ptr(), _ld(x2), w2.data_ptr(), _ld(w2), _lib.DT[x.dtype], M, N, K,
                   _lib.ptr(b), 0 if b is None else _lib.DT[b.dtype], _lib.ptr(res2), 0 if res2 is None else _ld(res2),
-                  ACTIVATIONS[activation], out2.data_ptr(), _ld(out2), _lib.stream_of(dev))
+                  ACTIVATIONS[activation], o_ptr, ldc, _lib.stream_of(dev))
     return target
 
 

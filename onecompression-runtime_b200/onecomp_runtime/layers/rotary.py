@@ -60,6 +60,24 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     return freq, gain
 
 
+def _in_place(what: str, t: torch.Tensor, T: int) -> tuple:
+    """Kernel arguments that rotate ``t`` [..., H, D] where it lies."""
+    H, D = t.shape[-2:]
+    try:
+        x = t if t.dim() == 3 else t.view(T, H, D)
+    except RuntimeError as e:
+        raise ValueError(f"{what}: in place needs token dimensions that fold into one stride, got strides "
+                         f"{t.stride()}") from e
+    st, sh, sd = x.stride()
+    if t.numel():
+        (s0, n0), (s1, n1) = sorted(((st, T), (sh, H)))
+        if D > 1 and sd != 1:
+            raise ValueError(f"{what}: in place needs a contiguous head, got strides {t.stride()}")
+        if (n0 > 1 and s0 < D) or (n1 > 1 and s1 < (max(s0 * (n0 - 1) + D, D) if n0 > 1 else D)):
+            raise ValueError(f"{what}: in place on overlapping rows (strides {t.stride()})")
+    return x.data_ptr(), st, sh, x.data_ptr(), st, sh, H
+
+
 class RotaryEmbedding(torch.nn.Module):
     """Rotates queries and keys by their positions (``oc_b200_rope``, one launch for both).
 
@@ -130,60 +148,50 @@ class RotaryEmbedding(torch.nn.Module):
         int64 [...], with ``axes`` [..., len(axes)]. Returns the rotated ``(q, k)``, rounded once; ``inplace``
         writes into the inputs (which may be slices of one projection's output)."""
         what = "RotaryEmbedding"
+        D = self.head_dim
         lead = q.shape[:-2]
         A = 1 if self.axes is None else len(self.axes)
-        want = (*lead, A) if self.axes is not None else tuple(lead)
+        want = lead if self.axes is None else (*lead, A)
         for name, t in (("q", q), ("k", k)):
-            if t is not None and (t.dim() < 3 or t.shape[:-2] != lead or t.shape[-1] != self.head_dim):
-                raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {(*lead, 'heads', self.head_dim)}")
-        if tuple(positions.shape) != want or positions.dtype not in (torch.int32, torch.int64):
+            if t is not None and (t.dim() < 3 or t.shape[:-2] != lead or t.shape[-1] != D):
+                raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {(*lead, 'heads', D)}")
+        if positions.shape != want or positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{what}: positions {positions.dtype} {tuple(positions.shape)}, expected int32 or int64 "
-                             f"{want}")
-        if q.dtype not in _lib.DT or (k is not None and k.dtype != q.dtype):
-            raise TypeError(f"{what} takes fp16, bf16 or fp32 of one dtype, got {q.dtype} and "
+                             f"{tuple(want)}")
+        dtype = q.dtype
+        if dtype not in _lib.DT or (k is not None and k.dtype != dtype):
+            raise TypeError(f"{what} takes fp16, bf16 or fp32 of one dtype, got {dtype} and "
                             f"{None if k is None else k.dtype}")
         inference_only(what, q, k)
         dev = one_device(what, q, k, positions)
-        T = math.prod(lead)
-        ins, outs, args = [], [], []
+        T = lead[0] if len(lead) == 1 else math.prod(lead)
+        sides = []   # per tensor: result, what the kernel reads, its arguments
         for t in (q, k):
             if t is None:
-                outs.append(None)
-                args += [None, 0, 0, None, 0, 0, 0]
-                continue
-            H = t.shape[-2]
-            if inplace:
-                try:
-                    src = t.view(T, H, self.head_dim)
-                except RuntimeError as e:
-                    raise ValueError(f"{what}: in place needs token dimensions that fold into one stride, got strides "
-                                     f"{t.stride()}") from e
-                if t.numel() and src.stride(2) != 1:
-                    raise ValueError(f"{what}: in place needs a contiguous head, got strides {t.stride()}")
-                (s0, n0), (s1, n1) = sorted(((src.stride(0), T), (src.stride(1), H)))
-                if t.numel() and ((n0 > 1 and s0 < self.head_dim) or (n1 > 1 and s1 < max(s0 * n0, self.head_dim))):
-                    raise ValueError(f"{what}: in place on overlapping rows (strides {t.stride()})")
-                dst, res = src, t
+                sides.append((None, None, (None, 0, 0, None, 0, 0, 0)))
+            elif inplace:
+                sides.append((t, t, _in_place(what, t, T)))
             else:
-                src = t.reshape(T, H, self.head_dim)
+                src = t if t.dim() == 3 else t.reshape(T, -1, D)
                 if src.stride(2) != 1:
                     src = src.contiguous()
-                dst = torch.empty((T, H, self.head_dim), dtype=t.dtype, device=dev)
-                res = dst.view(t.shape)
-            ins.append(src)
-            outs.append(res)
-            args += [src.data_ptr(), src.stride(0), src.stride(1), dst.data_ptr(), dst.stride(0), dst.stride(1), H]
+                res = torch.empty(t.shape, dtype=dtype, device=dev)
+                H = src.shape[1]
+                sides.append((res, src, (src.data_ptr(), src.stride(0), src.stride(1), res.data_ptr(), H * D, D, H)))
         if T == 0:
-            return tuple(outs)
+            return sides[0][0], sides[1][0]
         turns, axis = self._table(dev)
-        pos = positions.reshape(T, A)
-        if A > 1 and pos.stride(1) != 1:
-            pos = pos.contiguous()
+        pos, pos_st = positions, 1
+        if positions.dim() != 1 or positions.stride(0) != 1:
+            pos = positions.reshape(T, A)
+            if A > 1 and pos.stride(1) != 1:
+                pos = pos.contiguous()
+            pos_st = pos.stride(0)
         with on_device(dev):
-            _lib.call("oc_b200_rope", *args, _lib.DT[q.dtype], T, self.head_dim, self.rotary_dim, pos.data_ptr(),
-                      int(pos.dtype == torch.int64), pos.stride(0), turns.data_ptr(), _lib.ptr(axis), self.gain,
-                      int(self.layout == "interleaved"), _lib.stream_of(dev))
-        return tuple(outs)
+            _lib.call("oc_b200_rope", *sides[0][2], *sides[1][2], _lib.DT[dtype], T, D, self.rotary_dim, pos.data_ptr(),
+                      pos.dtype == torch.int64, pos_st, turns.data_ptr(), _lib.ptr(axis), self.gain,
+                      self.layout == "interleaved", _lib.stream_of(dev))
+        return sides[0][0], sides[1][0]
 
     def extra_repr(self) -> str:
         return (f"head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, layout={self.layout}, axes={self.axes}, "
