@@ -151,6 +151,65 @@ int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, o
   return launch_check("dense_gemm");
 }
 
+// Equal token tiles, a multiple of 32 tokens, at most 256.
+int dense_bt(int M) {
+  const int tiles = (M + 255) / 256;
+  return ((M + tiles - 1) / tiles + 31) / 32 * 32;
+}
+
+template <bool BF16, int ACT, bool RES>
+int launch_dense_tile(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& d, int dev,
+                      cudaStream_t stream) {
+  const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  oc::DenseTileParams p{};
+  p.d = d;
+  p.bt = dense_bt(d.M);
+  p.tiles_n = (d.N + 255) / 256;
+  p.tiles_m = (d.M + p.bt - 1) / p.bt;
+  const long long tiles = (long long)p.tiles_n * p.tiles_m;
+  if (tiles > INT_MAX / 2) return fail(OC_ERR_INVALID, "dense_gemm: %lld tiles", tiles);
+  p.tiles = (int)tiles;
+  p.tma_epi = d.vec;
+  CUtensorMap tw, tx, tc = {}, tr = {};
+  if (int rc = make_tmap_2d(&tw, dt, 2, w, d.K, d.N, (uint64_t)ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tmap_2d(&tx, dt, 2, x, d.K, d.M, (uint64_t)ldx * 2, 64, p.bt / 2, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  if (p.tma_epi) {
+    if (int rc = make_tmap_2d(&tc, dt, 2, d.out, d.N, d.M, (uint64_t)d.ldc * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    if (RES)
+      if (int rc = make_tmap_2d(&tr, dt, 2, d.residual, d.N, d.M, (uint64_t)d.ldr * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+  }
+  auto kern = oc::dense_tile_kernel<BF16, ACT, RES>;
+  if (int rc = set_smem(kern, oc::kDtSmem)) return rc;
+  const int pairs = (int)std::min<long long>(tiles, sm_count(dev) / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(oc::kDtThreads);
+  cfg.dynamicSmemBytes = oc::kDtSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (int rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, tw, tx, tc, tr, p), "dense_gemm (pairs)")) return rc;
+  return launch_check("dense_gemm (pairs)");
+}
+
+template <bool BF16, bool RES>
+int launch_dense_tile_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& p, int dev,
+                          cudaStream_t stream) {
+  switch (p.act) {
+    case OC_ACT_GELU_TANH: return launch_dense_tile<BF16, oc::kDenseGeluTanh, RES>(x, ldx, w, ldw, p, dev, stream);
+    case OC_ACT_GELU: return launch_dense_tile<BF16, oc::kDenseGelu, RES>(x, ldx, w, ldw, p, dev, stream);
+    case OC_ACT_SILU: return launch_dense_tile<BF16, oc::kDenseSilu, RES>(x, ldx, w, ldw, p, dev, stream);
+    case OC_ACT_RELU: return launch_dense_tile<BF16, oc::kDenseRelu, RES>(x, ldx, w, ldw, p, dev, stream);
+    default: return launch_dense_tile<BF16, oc::kDenseNone, RES>(x, ldx, w, ldw, p, dev, stream);
+  }
+}
+
 template <bool BF16>
 int launch_dense(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& p, int dev,
                  cudaStream_t stream) {
@@ -158,7 +217,8 @@ int launch_dense(const void* x, int64_t ldx, const void* w, int64_t ldw, const o
   if (p.M <= 32) return launch_dense_split<BF16, 32>(x, ldx, w, ldw, p, dev, stream);
   if (p.M <= 64) return launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream);
   if (p.M <= 128) return launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
-  return launch_dense_split<BF16, 256>(x, ldx, w, ldw, p, dev, stream);
+  return p.residual ? launch_dense_tile_act<BF16, true>(x, ldx, w, ldw, p, dev, stream)
+                    : launch_dense_tile_act<BF16, false>(x, ldx, w, ldw, p, dev, stream);
 }
 
 }  // namespace

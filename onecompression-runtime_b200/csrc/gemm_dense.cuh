@@ -208,4 +208,250 @@ __global__ void __launch_bounds__(kDsThreads)
   if (S > 1) cluster_sync_all();   // no CTA leaves while another reads its accumulator
 }
 
+// Many tokens: bound by the tensor pipe. Persistent pairs of CTAs (a cluster of two, one per SM) compute
+// 256 features x up to 256 tokens with cta_group::2 MMAs: each CTA holds its 128 features' weights and
+// half of the tokens' activations, so an SM moves 32 KB of shared memory per 128 x 256 x 64 product instead
+// of 48 KB. Features are the MMA's M and tokens its N: a ragged token count is split into equal tiles
+// of a multiple of 32 tokens (517 tokens: three of 192 instead of three of 256). The accumulator is double
+// buffered in TMEM, so four epilogue warps drain a tile while the next one is multiplied. Every epilogue
+// warp owns 32 features (its TMEM lanes) and moves [32 tokens x 32 features] pieces through its own four
+// buffers by TMA, residual pieces loaded two ahead; outputs or residuals that a tensor map cannot
+// describe are stored directly.
+constexpr int kDtThreads = 256;     // warp 0: TMA, 1: MMA, 4-7: epilogue
+constexpr int kDtStages = 6;
+constexpr int kDtBufs = 4;
+constexpr int kDtPiece = 32 * 32 * 2;
+constexpr int kDtStageBytes = 2 * 128 * 128;
+constexpr int kDtBars = 2 * kDtStages + 2 * 2 + 1 + 4 * kDtBufs;
+constexpr int kDtSmem = kDtStages * kDtStageBytes + 4 * kDtBufs * kDtPiece + 1024 + kDtBars * 8 + 16;
+static_assert(kDtSmem <= 232448, "shared memory per CTA");
+
+struct DenseTileParams {
+  DenseParams d;
+  int bt;                          // tokens of a tile, a multiple of 32 up to 256
+  int tiles_n, tiles_m, tiles;     // 256-feature tiles, token tiles
+  int tma_epi;
+};
+
+__device__ __forceinline__ void tc_mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Tile number -> (feature tile, token tile): bands of 8 feature tiles, so that the pairs running at one
+// time share both weights and activations in L2.
+__device__ __forceinline__ void dense_tile_at(const DenseTileParams& p, int tile, int& tn, int& tm) {
+  const int band = tile / (8 * p.tiles_m), in = tile - band * 8 * p.tiles_m;
+  const int width = min(8, p.tiles_n - band * 8);
+  tm = in / width;
+  tn = band * 8 + in - tm * width;
+}
+
+template <bool BF16, int ACT, bool RES>
+__device__ __forceinline__ void dense_piece(const uint32_t (&v)[32], float bias, uint16_t* e) {
+  constexpr int kOdt = BF16 ? kBF16 : kF16;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float y = dense_act(__uint_as_float(v[i]) + bias, ACT);
+    if constexpr (RES) y += bits_to_f32(e[i * 32], kOdt);
+    e[i * 32] = f32_to_bits(y, kOdt);
+  }
+}
+
+template <bool BF16, int ACT, bool RES>
+__global__ void __launch_bounds__(kDtThreads, 1)
+    dense_tile_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                      const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_r,
+                      const DenseTileParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi = smem + kDtStages * kDtStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + 4 * kDtBufs * kDtPiece);   // the leader's count both CTAs' loads
+  uint64_t* empty = full + kDtStages;
+  uint64_t* acc_full = empty + kDtStages;    // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2] the leader's: one arrival per epilogue warp of both CTAs
+  uint64_t* drain = acc_empty + 2;
+  uint64_t* res_full = drain + 1;            // [4 warps][kDtBufs]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(res_full + 4 * kDtBufs);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  const int warp = warp_id(), lane = lane_id();
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int tile0 = blockIdx.x / 2, step = gridDim.x / 2;
+  const int KB = (p.d.K + 63) / 64;
+  const int half = p.bt / 2;
+  const uint32_t x_bytes = half * 128;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kDtStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
+    mbar_init(drain, 1);
+    for (int i = 0; i < 4 * kDtBufs; ++i) mbar_init(&res_full[i], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+    if (p.tma_epi) tma_prefetch_desc(&tmap_c);
+    if (RES && p.tma_epi) tma_prefetch_desc(&tmap_r);
+  }
+  if (warp == 1) {
+    tmem_alloc_cg2(tmem_holder, 512);
+    tmem_relinquish_cg2();
+  }
+  tc_fence_before();
+  cluster_sync_all();   // both CTAs' barriers are there before a copy or an arrival crosses over
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < p.tiles; tile += step) {
+        int tn, tm;
+        dense_tile_at(p, tile, tn, tm);
+        const int f0 = tn * 256 + (int)rank * 128, t0 = tm * p.bt + (int)rank * half;
+        for (int kb = 0; kb < KB; ++kb, ++it) {
+          const int st = it % kDtStages;
+          if (!mbar_wait(&empty[st], ((it / kDtStages) & 1) ^ 1, abort_flag, kDevErrTmaEmpty)) { ok = false; break; }
+          if (leader) mbar_arrive_expect_tx(&full[st], 2 * (128 * 128 + x_bytes));
+          const uint32_t bar = mapa_shared(&full[st], 0);
+          uint8_t* base = smem + st * kDtStageBytes;
+          tma_load_2d_pair(base, &tmap_w, bar, kb * 64, f0);
+          tma_load_2d_pair(base + 128 * 128, &tmap_x, bar, kb * 64, t0);
+        }
+      }
+      // our copies signal the leader's barrier: wait until the pair's MMAs have released the stages
+      // we filled, then every copy has landed
+      for (int i = it > kDtStages ? it - kDtStages : 0; i < it; ++i)
+        mbar_drain(&empty[i % kDtStages], (i / kDtStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t idesc = make_idesc_f16(BF16, 256, p.bt);
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < p.tiles; tile += step, ++n) {
+        const int a = n & 1;
+        if (!mbar_wait_cluster_ns(&acc_empty[a], ((n >> 1) & 1) ^ 1, kDevErrAccEmpty, OC_WAIT_NS)) { *abort_flag = 1; break; }
+        tc_fence_after();
+        for (int kb = 0; kb < KB; ++kb, ++it) {
+          const int st = it % kDtStages;
+          if (!mbar_wait(&full[st], (it / kDtStages) & 1, abort_flag, kDevErrTmaFull)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t wa = smem_u32(smem + st * kDtStageBytes), xa = wa + 128 * 128;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma_ss_pair(tmem + a * 256, smem_desc_kmajor_sw128(wa + j * 32), smem_desc_kmajor_sw128(xa + j * 32),
+                           idesc, (kb | j) != 0 ? 1u : 0u);
+          tc_commit_pair(&empty[st], 0x3);
+        }
+        if (ok) tc_commit_pair(&acc_full[a], 0x3);
+      }
+      tc_commit_pair(drain, 0x1);
+      mbar_drain(drain, 0);
+    }
+  } else if (warp >= 4) {
+    const int q4 = warp & 3;
+    uint16_t* bufs = reinterpret_cast<uint16_t*>(epi) + q4 * (kDtBufs * kDtPiece / 2);
+    uint64_t* rbar = res_full + q4 * kDtBufs;
+    uint32_t piece = 0;              // running piece counter: buffer piece & 3
+    uint32_t pend = 0, pend_par = 0; // lane 0: residual loads in flight, their phases
+    int n = 0;
+    auto load_res = [&](uint32_t pc, int f0, int t0) {
+      const int b = pc & (kDtBufs - 1);
+      mbar_arrive_expect_tx(&rbar[b], kDtPiece);
+      tma_load_2d(bufs + b * (kDtPiece / 2), &tmap_r, &rbar[b], f0, t0);
+      pend |= 1u << b;
+      pend_par = (pend_par & ~(1u << b)) | (((pc / kDtBufs) & 1u) << b);
+    };
+    for (int tile = tile0; tile < p.tiles; tile += step, ++n) {
+      int tn, tm;
+      dense_tile_at(p, tile, tn, tm);
+      const int a = n & 1;
+      const int f0 = tn * 256 + (int)rank * 128 + q4 * 32, t0 = tm * p.bt;
+      const int f = f0 + lane;
+      const float bias = p.d.bias && f < p.d.N ? load_as_f32(p.d.bias, p.d.bias_dtype, f) : 0.f;
+      // pieces that hold anything: the ragged last tiles stop early
+      const int pieces = f0 < p.d.N ? (min(p.bt, p.d.M - t0) + 31) / 32 : 0;
+      if (p.tma_epi && lane == 0) {
+        bulk_wait_group_read<2>();   // the stores of pieces piece - 4 and - 3 have read their buffers
+        if (RES)
+          for (int c = 0; c < 2 && c < pieces; ++c) load_res(piece + c, f0, t0 + c * 32);
+      }
+      __syncwarp();
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[a], (n >> 1) & 1, abort_flag, kDevErrAccFull));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(a * 256);
+#pragma unroll 1
+      for (int c = 0; c < pieces; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 32), v);
+        if (p.tma_epi) {
+          const int b = piece & (kDtBufs - 1);
+          if (lane == 0 && c + 2 < pieces) {
+            bulk_wait_group_read<1>();   // the store of piece - 2 has read the buffer of piece + 2
+            if (RES) load_res(piece + 2, f0, t0 + (c + 2) * 32);
+          }
+          tc_wait_ld();
+          if constexpr (RES) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&rbar[b], (piece / kDtBufs) & 1, abort_flag, kDevErrResFull));
+            if (!ok) break;
+            if (lane == 0) pend &= ~(1u << b);
+          }
+          __syncwarp();
+          dense_piece<BF16, ACT, RES>(v, bias, bufs + b * (kDtPiece / 2) + lane);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmap_c, bufs + b * (kDtPiece / 2), f0, t0 + c * 32);
+            bulk_commit_group();
+          }
+          ++piece;
+        } else {
+          tc_wait_ld();
+          constexpr int kOdt = BF16 ? kBF16 : kF16;
+          if (f < p.d.N) {
+            const int rows = min(32, p.d.M - t0 - c * 32);
+            uint16_t* dst = p.d.out + (long long)(t0 + c * 32) * p.d.ldc + f;
+            const uint16_t* res = RES ? p.d.residual + (long long)(t0 + c * 32) * p.d.ldr + f : nullptr;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < rows) {
+                float y = dense_act(__uint_as_float(v[i]) + bias, ACT);
+                if constexpr (RES) y += bits_to_f32(res[i * p.d.ldr], kOdt);
+                dst[i * p.d.ldc] = f32_to_bits(y, kOdt);
+              }
+          }
+        }
+      }
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(&acc_empty[a], 0));
+    }
+    if (lane == 0) {
+      bulk_wait_group0();
+      for (int b = 0; b < kDtBufs; ++b)
+        if (pend & (1u << b)) mbar_drain(&rbar[b], (pend_par >> b) & 1u);
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync_all();   // neither CTA leaves, or frees TMEM, while the pair's MMAs or arrivals may touch it
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_cg2(tmem, 512);
+  }
+}
+
 }  // namespace oc
