@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
           return true;
         };
         // S(j + 1) overwrites the columns of P(j) (two tiles) or P(j - 1) (one tile): only once the
-        // product that reads them is done
+        // product that reads them is done (relying on the order of issue instead gave 1 %)
         auto pv_over = [&](int t, int j) {
           return mbar_wait(&pv_done[t], j & 1, abort_flag, kDevErrAccFull);
         };
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
           for (int j = 0; ok && j < w.nblk; ++j)
             for (int t = 0; ok && t < w.ntile; ++t) {
               if (j < w.nb[t]) ok = pv(t, j);
-              if (ok && j + 1 < w.nb[t]) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(t, j)) && qk(t, j + 1);
+              if (ok && j + 1 < w.nb[t]) ok = (DP == 64 || pv_over(t, j)) && qk(t, j + 1);
             }
         } else {
           if (w.nblk > 0) ok = ok && qk(0, 0);
@@ -397,7 +397,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       tc_fence_before();
       mbar_arrive(&p_full[b]);
     }
-    // the row's output
+    // the row's output. With one tile the last S was ready before the product before last was: that
+    // one is waited for first, or its phase would pass for the last one's.
+    if (!kTwo && ok && nb > 1) ok = mbar_wait(&pv_done[t], (nb - 2) & 1, abort_flag, kDevErrAccEmpty);
     if (ok && nb > 0) ok = mbar_wait(&pv_done[t], (nb - 1) & 1, abort_flag, kDevErrAccEmpty);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {

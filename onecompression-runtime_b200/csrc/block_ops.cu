@@ -10,9 +10,6 @@
 #include "rope.cuh"
 #include "attn_common.cuh"
 #include "attn_split.cuh"
-#ifndef OC_ATTN_IN_ORDER
-#define OC_ATTN_IN_ORDER 0
-#endif
 #include "attn_tile.cuh"
 #include "gemm_dense.cuh"
 

@@ -249,6 +249,22 @@ def test_attention_repeats_bit_for_bit(cuda_device):
             assert all(torch.equal(first, packed_attention(q, k, v, cu(dev, lq), cu(dev, lk))) for _ in range(5))
 
 
+def test_attention_wide_heads_many_times(cuda_device):
+    """One row tile per CTA (head size 256): the last product of a tile may run long after its scores were
+    ready, so the output is read only once both of the last two products are done. Many tiles, many times."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    lens = [256, 1, 129, 384, 255, 640]
+    q, k, v = randn(dev, sum(lens), 12, 256, seed=1, std=1.5), randn(dev, sum(lens), 4, 256, seed=2), randn(dev, sum(lens), 4, 256, seed=3)
+    c = cu(dev, lens)
+    starts = [sum(lens[:i]) for i in range(len(lens))]
+    for causal in (False, True):
+        want, tol = ref.attention(q, k, v, [(s, n, s, n) for s, n in zip(starts, lens)], causal, 256 ** -0.5)
+        for _ in range(40):
+            with torch.no_grad():
+                ref.check(packed_attention(q, k, v, c, c, causal=causal), want, tol, "wide heads")
+
+
 # ---------------------------------------------------------------------------------------- rotary
 def angles(dev, pos, freq):
     return pos.double() * torch.tensor(freq, dtype=torch.float64, device=dev)
