@@ -76,11 +76,16 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
   using Cfg = SplitCfg<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[kSplitWarps][kSplitRows], sm_l[kSplitWarps][kSplitRows];
+  __shared__ int sm_odd;   // an infinity or NaN was taken out of the item's values
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, tq = lane & 3;
   int* desc = p.desc + blockIdx.x * kSplitDescInts;
-  if (threadIdx.x == 0) desc[0] = 0;   // rows of the item this CTA begins and others finish
+  if (threadIdx.x == 0) {
+    sm_odd = 0;
+    desc[0] = 0;   // rows of the item this CTA begins and others finish
+  }
+  __syncthreads();
 
   // the call's units, then this CTA's run of them (every warp finds it for itself)
   long long total = 0;
@@ -122,6 +127,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
   const uint32_t ring_addr = smem_u32(ring);
   constexpr int kCh = DP / 8;                      // 16-byte chunks of a row
   constexpr int kIter = 16 * kCh / 32;             // chunks per lane of one 16-row matrix
+  constexpr int kStep = 32 / kCh;                  // rows from one of a lane's chunks to its next
 
   while (u < u_end) {
     while (u >= seq_begin + split_units(p, s)) {
@@ -139,26 +145,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     const int rows = (int)min((long long)kSplitRows, (long long)s.nq * p.G - row0);
     const int kbeg = blk0 * kSplitBlock, kend = min(s.nk, blk1 * kSplitBlock);
 
-    // this lane's two rows: last visible key, and the queries as A fragments
-    int limit[2];
-    uint32_t qa[DP / 16][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i;
-      const long long row = row0 + r;
-      const int tok = (int)(row / p.G);
-      const uint16_t* qr = p.q + (s.q0 + tok) * p.q_st + (kvh * p.G + row % p.G) * p.q_sh;
-      limit[i] = r < rows ? (p.causal ? min(kend - 1, tok + s.nk - s.nq) : kend - 1) : -1;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int col = ks * 16 + h * 8 + 2 * tq;
-          qa[ks][2 * h + i] = (r < rows && col < p.D) ? *reinterpret_cast<const uint32_t*>(qr + col) : 0u;
-        }
-    }
-    const int first_limit = p.causal ? (int)(row0 / p.G) + s.nk - s.nq : kend - 1;   // of the tile's first token
-
     float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -169,25 +155,53 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     const int slices = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
     // rows behind the last key and columns behind D are filled with zeros: a weight of zero times
     // whatever lies there must not reach the output
+    const int c_row = lane / kCh, c_ch = lane % kCh;
+    const bool c_in = c_ch * 8 < p.D;
+    const uint16_t* k_src = kb + (long long)(kbeg + c_row) * p.k_st + c_ch * 8;
+    const uint16_t* v_src = vb + (long long)(kbeg + c_row) * p.v_st + c_ch * 8;
     auto issue = [&](int sl, int stage) {
       if (sl < slices) {
-        const int key0 = kbeg + sl * 16;
-        const uint32_t dst = ring_addr + stage * Cfg::kStageBytes;
+        const uint16_t* ks = k_src + (long long)sl * 16 * p.k_st;
+        const uint16_t* vs = v_src + (long long)sl * 16 * p.v_st;
+        const uint32_t dst = ring_addr + stage * Cfg::kStageBytes + c_row * (DP * 2);
+        const int left = kend - kbeg - sl * 16 - c_row;   // rows this lane may still copy
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {
-          const int idx = i * 32 + lane, r = idx / kCh, ch = idx % kCh;
-          const bool ok = key0 + r < kend && ch * 8 < p.D;
-          const long long key = ok ? key0 + r : 0;
-          const int col = ok ? ch * 8 : 0;
-          const uint32_t off = dst + r * (DP * 2) + ((ch ^ (r & 7)) * 16);
-          cp_async16(off, (ok ? kb + key * p.k_st + col : p.k), ok);
-          cp_async16(off + Cfg::kKvBytes, (ok ? vb + key * p.v_st + col : p.v), ok);
+          const bool ok = c_in && i * kStep < left;
+          const uint32_t off = dst + i * kStep * (DP * 2) + ((c_ch ^ ((i * kStep + c_row) & 7)) * 16);
+          cp_async16(off, ok ? ks : p.k, ok);
+          cp_async16(off + Cfg::kKvBytes, ok ? vs : p.v, ok);
+          ks += kStep * p.k_st;
+          vs += kStep * p.v_st;
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < Cfg::kStages - 1; ++i) issue(warp + i * kSplitWarps, i);
+
+    // this lane's two rows: last visible key, and the queries as A fragments
+    int limit[2];
+    uint32_t qa[DP / 16][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = g + 8 * i;
+      const long long row = row0 + r;
+      const int tok = (int)(row / p.G);
+      const uint16_t* qr = p.q + (s.q0 + tok) * p.q_st + (kvh * p.G + row % p.G) * p.q_sh + 2 * tq;
+      limit[i] = r < rows ? (p.causal ? min(kend - 1, tok + s.nk - s.nq) : kend - 1) : -1;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = ks * 16 + h * 8;
+          qa[ks][2 * h + i] = (r < rows && col < p.D) ? *reinterpret_cast<const uint32_t*>(qr + col) : 0u;
+        }
+    }
+    // slices from edge_begin on hold keys that some row of the tile does not see
+    const int first_limit = p.causal ? (int)(row0 / p.G) + s.nk - s.nq : kend - 1;   // of the tile's first token
+    const int edge_begin = kbeg + max(0, min(first_limit + 1, kend) - kbeg) / 16 * 16;
+    const bool has_edge = first_limit < kend - 1;
     int stage = 0;
     for (int sl = warp; sl < slices; sl += kSplitWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 2) : "memory");
@@ -205,75 +219,71 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
         mma16816<BF16>(c[0], qa[ks], r[0], r[1]);
         mma16816<BF16>(c[1], qa[ks], r[2], r[3]);
       }
-      float corr[2];
-      uint32_t pa[4];
+      // The exponents' reference follows the running maximum only when it grew by more than 2^8 (weights
+      // up to 256 are as exact in 16 bits as weights up to 1): the output is rarely scaled.
+      float top[2];
       bool grew = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = m[i];
+        top[i] = m[i];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float& x = c[t][2 * i + e];
             x = key0 + t * 8 + 2 * tq + e <= limit[i] ? x * p.scale_log2 : -INFINITY;
-            mx = fmaxf(mx, x);
+            top[i] = fmaxf(top[i], x);
           }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        corr[i] = ex2(m[i] - ref);
-        grew |= mx != m[i];
-        m[i] = mx;
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float p0 = ex2(c[t][2 * i] - ref), p1 = ex2(c[t][2 * i + 1] - ref);
-          sum += p0 + p1;
-          pa[2 * t + i] = pack2_rn<BF16>(p0, p1);   // weights in [0, 1] as the product's 16-bit operand
-        }
-        l[i] = l[i] * corr[i] + sum;
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        grew |= top[i] - m[i] > 8.f;
       }
       if (__any_sync(0xffffffffu, grew)) {
+        float corr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          corr[i] = top[i] > m[i] ? ex2(m[i] - top[i]) : 1.f;
+          m[i] = fmaxf(m[i], top[i]);
+          l[i] *= corr[i];
+        }
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) {
           o[i][0] *= corr[0]; o[i][1] *= corr[0];
           o[i][2] *= corr[1]; o[i][3] *= corr[1];
         }
       }
-      // does a row of the tile see less than this slice? then a value it does not see may be
-      // infinite or NaN, and its weight of zero must not turn that into NaN
-      const bool edge = min(key0 + 15, kend - 1) > first_limit;
+      uint32_t pa[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float ref = m[i] == -INFINITY ? 0.f : m[i];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float p0 = ex2(c[t][2 * i] - ref), p1 = ex2(c[t][2 * i + 1] - ref);
+          l[i] += p0 + p1;
+          pa[2 * t + i] = pack2_rn<BF16>(p0, p1);   // the weights as the product's 16-bit operand
+        }
+      }
+      // A value that a row does not see may be infinite or NaN, and its weight of zero must not turn that
+      // into NaN: such values leave the slice, and the rows that see them add them at the end.
+      if (has_edge && key0 >= edge_begin) {
+        uint4* vsl = reinterpret_cast<uint4*>(ring + stage * Cfg::kStageBytes + Cfg::kKvBytes);
+#pragma unroll 1
+        for (int i = lane; i < 16 * kCh; i += 32) {
+          uint4 x = vsl[i];
+          if (nonfinite2<BF16>(x.x) || nonfinite2<BF16>(x.y) || nonfinite2<BF16>(x.z) || nonfinite2<BF16>(x.w)) {
+            vsl[i] = make_uint4(finite2<BF16>(x.x), finite2<BF16>(x.y), finite2<BF16>(x.z), finite2<BF16>(x.w));
+            sm_odd = 1;
+          }
+        }
+        __syncwarp();
+      }
 #pragma unroll
       for (int d2 = 0; d2 < DP / 16; ++d2) {
         uint32_t r[4];
         const int row = lane & 15, ch = d2 * 2 + (lane >> 4);
         ldsm_x4_trans(vs_addr + row * (DP * 2) + ((ch ^ (row & 7)) * 16), r);
-        bool odd = false;
-        if (edge) {
-          odd = nonfinite2<BF16>(r[0]) || nonfinite2<BF16>(r[1]) || nonfinite2<BF16>(r[2]) || nonfinite2<BF16>(r[3]);
-          odd = __any_sync(0xffffffffu, odd);
-          if (odd)
-            for (int i = 0; i < 4; ++i) r[i] = finite2<BF16>(r[i]);
-        }
         mma16816<BF16>(o[2 * d2], pa, r[0], r[1]);
         mma16816<BF16>(o[2 * d2 + 1], pa, r[2], r[3]);
-        if (odd) {   // the rows that do see such a value add it
-          for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int col = d2 * 16 + t * 8 + 2 * tq + e;
-                const int cc = (col >> 3) ^ (j & 7);
-                const uint16_t bits = *reinterpret_cast<const uint16_t*>(
-                    smem + (vs_addr - smem_u32(smem)) + j * (DP * 2) + cc * 16 + (col & 7) * 2);
-                if (nonfinite2<BF16>(bits))
-#pragma unroll
-                  for (int i = 0; i < 2; ++i)
-                    if (key0 + j <= limit[i]) o[2 * d2 + t][2 * i + e] += bits_to_f32(bits, BF16 ? kBF16 : kF16);
-              }
-        }
       }
       stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
     }
@@ -312,6 +322,15 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
         lsum += a * sm_l[w][r];
         acc.x += a * x.x; acc.y += a * x.y; acc.z += a * x.z; acc.w += a * x.w;
       }
+      if (has_edge && sm_odd) {
+        const int last = min(kend - 1, (int)((row0 + r) / p.G) + s.nk - s.nq);
+        for (int key = edge_begin; key <= last; ++key) {
+          const uint16_t* vr = vb + (long long)key * p.v_st + c4;
+          float* y = &acc.x;
+          for (int e = 0; e < 4; ++e)
+            if (c4 < p.D && nonfinite2<BF16>(vr[e])) y[e] += bits_to_f32(vr[e], BF16 ? kBF16 : kF16);
+        }
+      }
       if (whole) {
         if (c4 < p.D) {
           const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
@@ -337,6 +356,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
       desc[0] = rows;
     }
     __syncthreads();
+    if (has_edge && threadIdx.x == 0) sm_odd = 0;   // read above, written again by the next item's slices
+    if (has_edge) __syncthreads();
     u += blk1 - blk0;
   }
 }

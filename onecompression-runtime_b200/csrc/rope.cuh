@@ -9,7 +9,7 @@
 //
 // Bound by HBM: each value is read and written once. A block takes TB tokens, computes their
 // TB * R/2 sines and cosines once into shared memory (all heads of a token share them) and then
-// walks the heads, one unit of two 16-byte vectors (V pairs) per thread and four units in flight.
+// walks the heads, one unit of two 16-byte vectors (V pairs) per thread and two units in flight.
 #pragma once
 
 #include "common.cuh"
@@ -57,7 +57,7 @@ template <> struct RopeElem<kF32> {
 
 // V values per vector: 16 bytes, or 1 where sizes, strides or pointers do not allow vectors.
 template <int DT, int V, bool INTER, int TB>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const RopeParams p) {
   using El = RopeElem<DT>;
   using E = typename El::T;
   struct alignas(sizeof(E) * V) Vec { E e[V]; };
@@ -84,50 +84,56 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
   const int U = UR + (p.copy_rest ? (p.D - p.R) / (2 * V) : 0);
   const int h_begin = blockIdx.y * p.heads_per_block;
   const int nh = min(p.heads_per_block, p.t[0].H + p.t[1].H - h_begin);
-  const int total = nt * nh * U;
-  constexpr int kBatch = 4;
-  for (int base = threadIdx.x; base < total; base += kBatch * kRopeThreads) {
-    Vec a[kBatch], b[kBatch];
-    E* dst[kBatch];
-    int second[kBatch], trig[kBatch];   // distance of the pair's second vector; -1: copied unit
+  // a thread keeps its unit and walks (token, head) in steps of the heads that the block covers at once
+  const int width = min(U, kRopeThreads), rows = kRopeThreads / width;
+  const int hr = threadIdx.x / width;
+  if (hr >= min(rows, nh)) return;
+  constexpr int kBatch = 2;
+  for (int u = threadIdx.x - hr * width; u < U; u += width) {
+    const bool rot = u < UR;
+    const int col = rot ? (INTER ? 2 * u * V : u * V) : p.R + (u - UR) * 2 * V;
+    const int second = rot && !INTER ? P : V;   // distance of the pair's second vector
+    int t = 0, h = hr;
+    while (t < nt) {
+      Vec a[kBatch], b[kBatch];
+      E* dst[kBatch];
+      int trig[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int i = base + j * kRopeThreads;
-      dst[j] = nullptr;
-      if (i >= total) continue;
-      const int th = i / U, u = i - th * U;
-      const int t = th / nh;
-      int h = h_begin + (th - t * nh);
-      const bool is_k = h >= p.t[0].H;
-      const RopeTensor& x = p.t[is_k ? 1 : 0];
-      if (is_k) h -= p.t[0].H;
-      const bool rot = u < UR;
-      const int col = rot ? (INTER ? 2 * u * V : u * V) : p.R + (u - UR) * 2 * V;
-      second[j] = rot && !INTER ? P : V;
-      trig[j] = rot ? t * P + u * V : -1;
-      const E* src = reinterpret_cast<const E*>(x.x) + (t0 + t) * x.xst + h * x.xsh + col;
-      dst[j] = reinterpret_cast<E*>(x.y) + (t0 + t) * x.yst + h * x.ysh + col;
-      a[j] = *reinterpret_cast<const Vec*>(src);
-      b[j] = *reinterpret_cast<const Vec*>(src + second[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (!dst[j]) continue;
-      if (trig[j] >= 0) {
-        const float* c = cs + trig[j];
-        const float* s = sn + trig[j];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          // half layout: pair e is (a[e], b[e]); interleaved: neighbours of the 2V values a, b
-          E& e1 = INTER ? (2 * e < V ? a[j].e[(2 * e) % V] : b[j].e[(2 * e) % V]) : a[j].e[e];
-          E& e2 = INTER ? (2 * e + 1 < V ? a[j].e[(2 * e + 1) % V] : b[j].e[(2 * e + 1) % V]) : b[j].e[e];
-          const float x1 = El::get(e1), x2 = El::get(e2);
-          e1 = El::put(x1 * c[e] - x2 * s[e]);
-          e2 = El::put(x2 * c[e] + x1 * s[e]);
+      for (int j = 0; j < kBatch; ++j) {
+        dst[j] = nullptr;
+        if (t < nt) {
+          const int hh = h_begin + h;
+          const bool is_k = hh >= p.t[0].H;
+          const RopeTensor& x = p.t[is_k ? 1 : 0];
+          const long long hx = is_k ? hh - p.t[0].H : hh;
+          const E* src = reinterpret_cast<const E*>(x.x) + (t0 + t) * x.xst + hx * x.xsh + col;
+          dst[j] = reinterpret_cast<E*>(x.y) + (t0 + t) * x.yst + hx * x.ysh + col;
+          trig[j] = t * P + u * V;
+          a[j] = *reinterpret_cast<const Vec*>(src);
+          b[j] = *reinterpret_cast<const Vec*>(src + second);
+          h += rows;
+          if (h >= nh) { h = hr; ++t; }
         }
       }
-      *reinterpret_cast<Vec*>(dst[j]) = a[j];
-      *reinterpret_cast<Vec*>(dst[j] + second[j]) = b[j];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (!dst[j]) continue;
+        if (rot) {
+          const float* c = cs + trig[j];
+          const float* s = sn + trig[j];
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            // half layout: pair e is (a[e], b[e]); interleaved: neighbours of the 2V values a, b
+            E& e1 = INTER ? (2 * e < V ? a[j].e[(2 * e) % V] : b[j].e[(2 * e) % V]) : a[j].e[e];
+            E& e2 = INTER ? (2 * e + 1 < V ? a[j].e[(2 * e + 1) % V] : b[j].e[(2 * e + 1) % V]) : b[j].e[e];
+            const float x1 = El::get(e1), x2 = El::get(e2);
+            e1 = El::put(x1 * c[e] - x2 * s[e]);
+            e2 = El::put(x2 * c[e] + x1 * s[e]);
+          }
+        }
+        *reinterpret_cast<Vec*>(dst[j]) = a[j];
+        *reinterpret_cast<Vec*>(dst[j] + second) = b[j];
+      }
     }
   }
 }
