@@ -71,6 +71,85 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Bounded wait (mbar_wait) of a whole warp with one result for all of it: code that stays uniform over
+// the warp keeps descriptors and counters in uniform registers, which the tensor instructions read.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((it & 15u) == 0u && __any_sync(0xffffffffu, *abort_flag != 0 || global_timer_ns() - t0 > OC_WAIT_NS)) break;
+  }
+  if (lane_id() == 0 && !*abort_flag) record_error(code);
+  __syncwarp();
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+template <typename T> __device__ __forceinline__ T warp_uniform(T v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Pairs of fp32 values in one 64-bit register (the FMA pipe takes both halves in one issue slot).
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of a pair on the FMA pipe, beside the 16 a cycle and SM that ex2.approx gives: x = n + f with n the
+// nearest integer (the magic sum 1.5 2^23 + x keeps n in its low bits), 2^f on [-1/2, 1/2] by the
+// polynomial of degree 4 with the least largest relative error (Remez exchange; 2.6e-6), times 2^n built
+// in the exponent field. NaN stays NaN; x is clamped to -126 from below, x above 127 does not occur.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  float a, b;
+  f2_unpack(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = f2_pack(a, b);
+  const uint64_t magic = f2_pack(12582912.f, 12582912.f), neg = f2_pack(-12582912.f, -12582912.f);
+  const uint64_t n = f2_add(x, magic);
+  const uint64_t f = f2_fma(f2_add(n, neg), f2_pack(-1.f, -1.f), x);
+  uint64_t r = f2_pack(0.009570102207362652f, 0.009570102207362652f);
+  r = f2_fma(r, f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
+  r = f2_fma(r, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+  r = f2_fma(r, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+  r = f2_fma(r, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+  f2_unpack(n, a, b);
+  const float sa = __int_as_float((__float_as_int(a) << 23) + 0x3f800000);
+  const float sb = __int_as_float((__float_as_int(b) << 23) + 0x3f800000);
+  return f2_mul(r, f2_pack(sa, sb));
+}
+
 // Is one of the two 16-bit values of a register infinite or NaN?
 template <bool BF16> __device__ __forceinline__ bool nonfinite2(uint32_t v) {
   constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;

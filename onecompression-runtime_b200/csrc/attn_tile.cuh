@@ -6,7 +6,9 @@
 // keys in blocks of 128.
 //   * A softmax warpgroup per tile, one thread per row: it reads S from TMEM (no shuffles), writes the
 //     16-bit weights P back to TMEM as the A operand of the second product, and keeps maximum and sum
-//     in registers. While one tile is in its softmax the tensor pipe runs the other tile's products.
+//     in registers. Each tile's products are issued by a thread of their own: while one tile is in its
+//     softmax the tensor pipe runs the other's, and the second product starts on the first 64 keys'
+//     weights while the softmax works on the rest.
 //   * The reference that the exponents are taken against follows the running maximum only when
 //     it grows by more than 2^8: weights up to 256 are as exact in 16 bits as weights up to 1, and
 //     the accumulator in TMEM is read, scaled and written back only in those rare steps.
@@ -22,6 +24,8 @@
 // causal tiles start first. All waits are bounded (common.cuh).
 #pragma once
 
+#include <type_traits>
+
 #include "attn_common.cuh"
 
 namespace oc {
@@ -29,23 +33,37 @@ namespace oc {
 constexpr int kTileKeys = 128;
 constexpr int kTileUnitBytes = 128 * 128;   // [128 rows x 64 columns] of 16-bit values
 constexpr int kTileMaxEdges = 3;
+#ifndef OC_ATTN_POLY
+#define OC_ATTN_POLY 0
+#endif
+#ifndef OC_ATTN_PART
+#define OC_ATTN_PART 3
+#endif
+#ifndef OC_ATTN_IN_ORDER
+#define OC_ATTN_IN_ORDER 0
+#endif
+constexpr int kTilePart = OC_ATTN_PART;     // of 4 chunks of 32 keys, those whose product starts ahead of the rest
+constexpr int kTilePoly = OC_ATTN_POLY;     // of 16 pairs of exponentials, those on the FMA pipe
 
 template <int DP> struct TileCfg {
   static constexpr int kTiles = DP == 256 ? 1 : 2;          // row tiles of a CTA
   static constexpr int kRows = kTiles * 128;
   static constexpr int kUnits = DP / 64;                    // units of a K or V block
   static constexpr int kSlots = DP == 256 ? 2 : DP == 128 ? 5 : 10;
+  static constexpr int kGroup = DP == 256 ? 1 : kUnits;     // units that share a barrier: few blocks fit at 256,
+                                                            // where loads follow the products unit by unit
+  static constexpr int kGroups = kUnits / kGroup;
   static constexpr int kSoftmaxThreads = kTiles * 128;
   static constexpr int kThreads = kSoftmaxThreads + 128;
   static constexpr int kQBytes = kTiles * kUnits * kTileUnitBytes;
   static constexpr int kRingBytes = kSlots * kUnits * kTileUnitBytes;
-  static constexpr int kBars = 2 * kSlots * kUnits + 1 + 2 + 2 + 2 + 2 * kTileMaxEdges + 1;
+  static constexpr int kBars = 2 * kSlots * kGroups + 1 + 2 + 2 + 2 + 2 + 2 * kTileMaxEdges + 1;
   static constexpr int kSmem = kQBytes + kRingBytes + 1024 + kBars * 8 + 32;
   static constexpr uint32_t kOCol = 256;
-  __device__ static uint32_t s_col(int i) { return i * 128; }
+  __device__ static constexpr uint32_t s_col(int i) { return i * 128; }
   // P shares the columns of its S (read by then), except where the head leaves TMEM to spare
-  __device__ static uint32_t p_col(int i) { return DP == 64 ? 384 + i * 64 : i * 128; }
-  __device__ static uint32_t o_col(int t) { return kOCol + t * DP; }
+  __device__ static constexpr uint32_t p_col(int i) { return DP == 64 ? 384 + i * 64 : i * 128; }
+  __device__ static constexpr uint32_t o_col(int t) { return kOCol + t * DP; }
   static_assert(kSmem <= 232448, "shared memory per CTA");
 };
 
@@ -125,17 +143,18 @@ template <bool BF16, int DP>
 __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const int n_slots, const int negate) {
   using Cfg = TileCfg<DP>;
-  constexpr int U = Cfg::kUnits, NU = Cfg::kSlots * U;
+  constexpr int U = Cfg::kUnits, GU = Cfg::kGroup, GN = Cfg::kGroups, NB = Cfg::kSlots * GN;
   constexpr bool kTwo = Cfg::kTiles == 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = smem;
   uint8_t* ring = smem + Cfg::kQBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + Cfg::kRingBytes);
-  uint64_t* empty = full + NU;
-  uint64_t* q_full = empty + NU;
+  uint64_t* empty = full + NB;
+  uint64_t* q_full = empty + NB;
   uint64_t* s_full = q_full + 1;            // [2] by tile, or by block parity where there is one tile
-  uint64_t* p_full = s_full + 2;            // [2]
+  uint64_t* p_part = s_full + 2;            // [2] the first 32 * kTilePart keys' weights are there
+  uint64_t* p_full = p_part + 2;            // [2] all are
   uint64_t* pv_done = p_full + 2;           // [2] by tile
   uint64_t* edge_full = pv_done + 2;        // [3] V blocks from e0 on: loaded
   uint64_t* edge_ready = edge_full + kTileMaxEdges;   // [3] and prepared
@@ -143,7 +162,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   volatile int* odd_values = abort_flag + 1;   // an infinity or NaN was taken out of a V block
-  const int warp = warp_id(), lane = lane_id();
+  const int warp = warp_uniform(warp_id()), lane = lane_id();
 
   if (p.zero_tail) attn_zero_tail(p, blockIdx.x, gridDim.x);
   if (blockIdx.x == 0)
@@ -154,9 +173,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   const int off = s.nk - s.nq;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NU; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < NB; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_part[i], 128); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1); }
     for (int i = 0; i < kTileMaxEdges; ++i) { mbar_init(&edge_full[i], 1); mbar_init(&edge_ready[i], 64); }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -198,8 +217,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
             mbar_arrive_expect_tx(&edge_full[j - w.e0], U * kTileUnitBytes);
             ++edges;
           }
-          for (int u = 0; u < U; ++u) {
-            const int i = slot * U + u;
+          for (int g = 0; g < GN; ++g) {
+            const int i = slot * GN + g;
             if (!mbar_wait(&empty[i], par ^ 1, abort_flag, kDevErrTmaEmpty)) {
               // an edge block was announced: its remaining bytes never come, so nobody drains it
               if (edge) --edges;
@@ -208,84 +227,112 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
             }
             uint64_t* bar = edge ? &edge_full[j - w.e0] : &full[i];
             if (edge) mbar_arrive(&full[i]);   // the ring's phases go on; the block is announced on its own barrier
-            else mbar_arrive_expect_tx(&full[i], kTileUnitBytes);
-            tma_load_3d(ring + i * kTileUnitBytes, is_v ? &maps.v : &maps.k, bar, u * 64, w.kvh, s.k0 + j * kTileKeys);
+            else mbar_arrive_expect_tx(&full[i], GU * kTileUnitBytes);
+            for (int u = g * GU; u < (g + 1) * GU; ++u)
+              tma_load_3d(ring + (slot * U + u) * kTileUnitBytes, is_v ? &maps.v : &maps.k, bar, u * 64, w.kvh,
+                          s.k0 + j * kTileKeys);
             ++uses;
           }
         }
         // every load issued lands before the CTA exits (consumed ones return at once)
         mbar_drain(q_full, 0);
-        for (int i = uses > NU ? uses - NU : 0; i < uses; ++i) mbar_drain(&full[i % NU], (i / NU) & 1);
+        for (int i = uses > NB ? uses - NB : 0; i < uses; ++i) mbar_drain(&full[i % NB], (i / NB) & 1);
         for (int e = 0; e < edges; ++e) mbar_drain(&edge_full[e], 0);
       }
     } else if (warp == kAux + 1) {
       // ------------------------------------------------------------ MMA
-      if (lane == 0) {
-        const uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128) | (negate ? 1u << 13 : 0u);
-        constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, DP) | (1u << 16);   // B is MN-major
-        const int last_tile = w.ntile - 1;
-        auto qk = [&](int t, int j) {
-          const int n = k_use<DP>(j), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
-          const int b = kTwo ? t : (j & 1);
-          for (int u = 0; u < U; ++u) {
-            const int i = slot * U + u;
-            if (!mbar_wait(&full[i], par, abort_flag, kDevErrTmaFull)) return false;
-            tc_fence_after();
-            const uint32_t qa = smem_u32(q_smem + (t * U + u) * kTileUnitBytes), ka = smem_u32(ring + i * kTileUnitBytes);
+      // The whole warp runs this with warp-uniform values; one elected thread issues.
+      const uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128) | (negate ? 1u << 13 : 0u);
+      constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, DP) | (1u << 16);   // B is MN-major
+      const int last_tile = warp_uniform(w.ntile - 1), nblk = warp_uniform(w.nblk), e0 = warp_uniform(w.e0);
+      const int nb0 = warp_uniform(w.nb[0]);
+      const uint32_t tm = warp_uniform(tmem);
+      const uint64_t q_desc = smem_desc_kmajor_sw128(smem_u32(q_smem));
+      const uint64_t k_desc = smem_desc_kmajor_sw128(smem_u32(ring)), v_desc = smem_desc_mnmajor_sw128(smem_u32(ring));
+      // `first`: no other tile has waited for the block yet
+      auto qk = [&](const int t, const int j, const bool first) {
+        const int n = k_use<DP>(j), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
+        const int b = kTwo ? t : (j & 1);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc_mma_ss(tmem + Cfg::s_col(b), smem_desc_kmajor_sw128(qa + k * 32), smem_desc_kmajor_sw128(ka + k * 32),
-                        idesc_qk, (u | k) != 0 ? 1u : 0u);
-            if (t == last_tile) tc_commit(&empty[i]);
-          }
-          tc_commit(&s_full[b]);
-          return true;
-        };
-        auto pv = [&](int t, int j) {
-          const int n = v_use<DP>(j, w.nblk), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
-          const int b = kTwo ? t : (j & 1);
-          if (j >= w.e0) {
-            if (!mbar_wait(&edge_ready[j - w.e0], 0, abort_flag, kDevErrWFull)) return false;
-          } else {
-            for (int u = 0; u < U; ++u)
-              if (!mbar_wait(&full[slot * U + u], par, abort_flag, kDevErrTmaFull)) return false;
-          }
-          if (!mbar_wait(&p_full[b], kTwo ? (j & 1) : ((j >> 1) & 1), abort_flag, kDevErrAFull)) return false;
+        for (int g = 0; g < GN; ++g) {
+          if (first && !mbar_wait_warp(&full[slot * GN + g], par, abort_flag, kDevErrTmaFull)) return false;
           tc_fence_after();
-          const uint32_t va = smem_u32(ring + slot * U * kTileUnitBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            tc_mma_ts(tmem + Cfg::o_col(t), tmem + Cfg::p_col(b) + k * 8, smem_desc_mnmajor_sw128(va + k * 2048),
-                      idesc_pv, (j | k) != 0 ? 1u : 0u);
-          if (t == last_tile)
-            for (int u = 0; u < U; ++u) tc_commit(&empty[slot * U + u]);
-          tc_commit(&pv_done[t]);
-          return true;
-        };
-        // S(j + 1) overwrites the columns of P(j) (two tiles) or P(j - 1) (one tile): only once the
-        // product that reads them is done (relying on the order of issue instead gave 1 %)
-        auto pv_over = [&](int t, int j) {
-          return mbar_wait(&pv_done[t], j & 1, abort_flag, kDevErrAccFull);
-        };
-        bool ok = mbar_wait(q_full, 0, abort_flag, kDevErrResFull);
-        if constexpr (kTwo) {
-          for (int t = 0; ok && t < w.ntile; ++t)
-            if (w.nb[t] > 0) ok = qk(t, 0);
-          for (int j = 0; ok && j < w.nblk; ++j)
-            for (int t = 0; ok && t < w.ntile; ++t) {
-              if (j < w.nb[t]) ok = pv(t, j);
-              if (ok && j + 1 < w.nb[t]) ok = (DP == 64 || pv_over(t, j)) && qk(t, j + 1);
-            }
-        } else {
-          if (w.nblk > 0) ok = ok && qk(0, 0);
-          for (int j = 0; ok && j < w.nblk; ++j) {
-            if (j + 1 < w.nblk) ok = (j == 0 || pv_over(0, j - 1)) && qk(0, j + 1);
-            if (ok) ok = pv(0, j);
+            for (int u = g * GU; u < (g + 1) * GU; ++u)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)   // descriptors count in units of 16 bytes
+                tc_mma_ss(tm + Cfg::s_col(b), q_desc + (t * U + u) * (kTileUnitBytes / 16) + k * 2,
+                          k_desc + (slot * U + u) * (kTileUnitBytes / 16) + k * 2, idesc_qk, (u | k) != 0 ? 1u : 0u);
+            if (g == GN - 1) tc_commit(&s_full[b]);
+            if (t == last_tile) tc_commit(&empty[slot * GN + g]);
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      auto pv = [&](const int t, const int j, const bool first) {
+        const int n = v_use<DP>(j, nblk), slot = n % Cfg::kSlots, par = (n / Cfg::kSlots) & 1;
+        const int b = kTwo ? t : (j & 1);
+        const uint32_t pp = kTwo ? (j & 1) : ((j >> 1) & 1);
+        if (first) {
+          if (j >= e0) {
+            if (!mbar_wait_warp(&edge_ready[j - e0], 0, abort_flag, kDevErrWFull)) return false;
+          } else {
+#pragma unroll
+            for (int g = 0; g < GN; ++g)
+              if (!mbar_wait_warp(&full[slot * GN + g], par, abort_flag, kDevErrTmaFull)) return false;
           }
         }
+        const uint64_t vd = v_desc + slot * U * (kTileUnitBytes / 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {   // the first keys' weights while the softmax still works on the others
+          if (!mbar_wait_warp(h ? &p_full[b] : &p_part[b], pp, abort_flag, kDevErrAFull)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = h ? 2 * kTilePart : 0; k < (h ? 8 : 2 * kTilePart); ++k)
+              tc_mma_ts(tm + Cfg::o_col(t), tm + Cfg::p_col(b) + k * 8, vd + k * (2048 / 16), idesc_pv,
+                        (j | k) != 0 ? 1u : 0u);
+            if (h) {
+              tc_commit(&pv_done[t]);
+              if (t == last_tile)
+#pragma unroll
+                for (int g = 0; g < GN; ++g) tc_commit(&empty[slot * GN + g]);
+            }
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      // S(j + 1) overwrites the columns of P(j) (two tiles) or P(j - 1) (one tile): only once the
+      // product that reads them is done
+      auto pv_over = [&](const int t, const int j) {
+        return mbar_wait_warp(&pv_done[t], j & 1, abort_flag, kDevErrAccFull);
+      };
+      bool ok = mbar_wait_warp(q_full, 0, abort_flag, kDevErrResFull);
+      if constexpr (kTwo) {
+        if (ok && nb0 > 0) ok = qk(0, 0, true);
+        if (ok && last_tile && nblk > 0) ok = qk(1, 0, nb0 == 0);
+        for (int j = 0; ok && j < nblk; ++j) {
+          if (j < nb0) ok = pv(0, j, true);
+          if (ok && j + 1 < nb0) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(0, j)) && qk(0, j + 1, true);
+          if (!last_tile) continue;
+          if (ok) ok = pv(1, j, j >= nb0);
+          if (ok && j + 1 < nblk) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(1, j)) && qk(1, j + 1, j + 1 >= nb0);
+        }
+      } else {
+        if (nblk > 0) ok = ok && qk(0, 0, true);
+        for (int j = 0; ok && j < nblk; ++j) {
+          if (j + 1 < nblk) ok = (j == 0 || pv_over(0, j - 1)) && qk(0, j + 1, true);
+          if (ok) ok = pv(0, j, true);
+        }
+      }
+      if (elect_one()) {
         tc_commit(drain);
         mbar_drain(drain, 0);
       }
+      __syncwarp();
     } else {
       // ------------------------------------------------------------ V blocks at the end of what rows see
       const int tid = threadIdx.x - (kAux + 2) * 32;
@@ -338,7 +385,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tmem + lanes + Cfg::s_col(b) + c * 32, v[c]);
       tc_wait_ld();
-      if (j * kTileKeys + kTileKeys - 1 > limit0) {
+      const bool edge = j * kTileKeys + kTileKeys - 1 > limit0;   // some row of the warp does not see all
+      if (edge) {
         const int seen = limit - j * kTileKeys;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -349,11 +397,11 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(v[c][0]);
+        mx[c] = m;
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+        for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
       }
-      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+      const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
       if (j == 0) {
         m = top;
       } else {
@@ -378,24 +426,44 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         }
       }
       const float bias = m == -INFINITY ? 0.f : -m * sc;
-      float sum[2] = {0.f, 0.f};
+      const uint64_t sc2 = f2_pack(sc, sc), bias2 = f2_pack(bias, bias);
+      uint64_t sum = 0;   // (0.f, 0.f)
+      // Of every 16 pairs kTilePoly go through the polynomial, so that neither the exponential unit nor
+      // the FMA pipe is waited for; blocks with masked scores take ex2, which gives them exact zeros.
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = ex2(fmaf(__uint_as_float(v[c][2 * i]), sc, bias));
-          const float p1 = ex2(fmaf(__uint_as_float(v[c][2 * i + 1]), sc, bias));
-          sum[0] += p0;
-          sum[1] += p1;
-          pk[i] = pack2_rn<BF16>(p0, p1);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x =
+                f2_fma(f2_pack(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, bias2);
+            float p0, p1;
+            uint64_t w2;
+            if (poly && i * kTilePoly % 16 < kTilePoly) {
+              w2 = ex2_poly2(x);
+              f2_unpack(w2, p0, p1);
+            } else {
+              f2_unpack(x, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              w2 = f2_pack(p0, p1);
+            }
+            sum = f2_add(sum, w2);
+            pk[i] = pack2_rn<BF16>(p0, p1);
+          }
+          tmem_st_32x32b_x16(tmem + lanes + Cfg::p_col(b) + c * 16, pk);
+          if (c == kTilePart - 1 || c == 3) {
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(c == 3 ? &p_full[b] : &p_part[b]);
+          }
         }
-        tmem_st_32x32b_x16(tmem + lanes + Cfg::p_col(b) + c * 16, pk);
-      }
-      l += sum[0] + sum[1];
-      tc_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[b]);
+      };
+      if (edge) weights(std::false_type{}); else weights(std::true_type{});
+      float s0, s1;
+      f2_unpack(sum, s0, s1);
+      l += s0 + s1;
     }
     // the row's output. With one tile the last S was ready before the product before last was: that
     // one is waited for first, or its phase would pass for the last one's.
