@@ -5,6 +5,7 @@ over packed sequences, and the dense 16-bit linear with its epilogue.
 ``onecomp_runtime``. Sizes follow the framework's own workloads: 32 heads of 128 (hidden 4096, fc1 16384)
 of the video-DiT stack, the 5120-wide decode layers; wide heads rotated in part are the other common form.
 """
+import functools
 import math
 import random
 import sys
@@ -17,8 +18,9 @@ own = False
 _DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
+@functools.lru_cache(maxsize=None)
 def _layers():
-    """The framework's layers; the package lies one folder below the repository's root."""
+    """The framework's layers, imported once; the package lies one folder below the repository's root."""
     root = str(Path(__file__).resolve().parents[1] / "onecompression-runtime_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
