@@ -71,31 +71,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Bounded wait (mbar_wait) of a whole warp with one result for all of it: code that stays uniform over
-// the warp keeps descriptors and counters in uniform registers, which the tensor instructions read.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned code) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = global_timer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    if ((it & 15u) == 0u && __any_sync(0xffffffffu, *abort_flag != 0 || global_timer_ns() - t0 > OC_WAIT_NS)) break;
-  }
-  if (lane_id() == 0 && !*abort_flag) record_error(code);
-  __syncwarp();
-  *abort_flag = 1;
-  return false;
-}
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r));
-  return r != 0;
-}
-template <typename T> __device__ __forceinline__ T warp_uniform(T v) { return __shfl_sync(0xffffffffu, v, 0); }
-
 // Pairs of fp32 values in one 64-bit register (the FMA pipe takes both halves in one issue slot).
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
   uint64_t r;

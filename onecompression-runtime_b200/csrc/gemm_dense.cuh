@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kDsThreads)
   uint64_t* done = empty + Cfg::kStages;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  const int warp = warp_id(), lane = lane_id();
+  const int warp = warp_uniform(warp_id()), lane = lane_id();
   uint32_t rank, S;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(S));
@@ -94,38 +94,43 @@ __global__ void __launch_bounds__(kDsThreads)
   const uint32_t tmem = *tmem_holder;
 
   if (warp == 4) {
-    if (lane == 0) {
+    const bool leader = elect_one();
+    if (leader) {
       tma_prefetch_desc(&tmap_w);
       tma_prefetch_desc(&tmap_x);
-      int it = 0;
-      for (; it < nkb; ++it) {
-        const int st = it % Cfg::kStages;
-        if (!mbar_wait(&empty[st], ((it / Cfg::kStages) & 1) ^ 1, abort_flag, kDevErrTmaEmpty)) break;
+    }
+    int it = 0;
+    for (int st = 0, par = 1; it < nkb; ++it) {
+      if (!mbar_wait_warp(&empty[st], par, abort_flag, kDevErrTmaEmpty)) break;
+      if (leader) {
         uint8_t* base = smem + st * Cfg::kStageBytes;
         mbar_arrive_expect_tx(&full[st], Cfg::kStageBytes);
         tma_load_2d(base, &tmap_w, &full[st], (kb0 + it) * 64, n0);
         tma_load_2d(base + Cfg::kWBytes, &tmap_x, &full[st], (kb0 + it) * 64, m0);
       }
-      // every load issued lands before the CTA goes on (consumed ones return at once)
+      if (++st == Cfg::kStages) { st = 0; par ^= 1; }
+    }
+    // every load issued lands before the CTA goes on (consumed ones return at once)
+    if (leader)
       for (int i = it > Cfg::kStages ? it - Cfg::kStages : 0; i < it; ++i)
         mbar_drain(&full[i % Cfg::kStages], (i / Cfg::kStages) & 1);
-    }
   } else if (warp == 5) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_f16(BF16, 128, BN);
-      for (int it = 0; it < nkb; ++it) {
-        const int st = it % Cfg::kStages;
-        if (!mbar_wait(&full[st], (it / Cfg::kStages) & 1, abort_flag, kDevErrTmaFull)) break;
-        tc_fence_after();
-        const uint32_t wa = smem_u32(smem + st * Cfg::kStageBytes), xa = wa + Cfg::kWBytes;
+    constexpr uint32_t idesc = make_idesc_f16(BF16, 128, BN);
+    const uint32_t tm = warp_uniform(tmem);
+    const uint64_t desc = smem_desc_kmajor_sw128(smem_u32(smem));   // counts in units of 16 bytes
+    const bool leader = elect_one();
+    for (int it = 0, st = 0, par = 0; it < nkb; ++it) {
+      if (!mbar_wait_warp(&full[st], par, abort_flag, kDevErrTmaFull)) break;
+      tc_fence_after();
+      const uint64_t wd = desc + st * (Cfg::kStageBytes / 16), xd = wd + Cfg::kWBytes / 16;
+      if (leader) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          tc_mma_ss(tmem, smem_desc_kmajor_sw128(wa + j * 32), smem_desc_kmajor_sw128(xa + j * 32), idesc,
-                    (it | j) != 0 ? 1u : 0u);
+        for (int j = 0; j < 4; ++j) tc_mma_ss(tm, wd + j * 2, xd + j * 2, idesc, (it | j) != 0 ? 1u : 0u);
         tc_commit(&empty[st]);
       }
-      tc_commit(done);
+      if (++st == Cfg::kStages) { st = 0; par ^= 1; }
     }
+    if (leader) tc_commit(done);
   }
   __syncwarp();
   bool ok = true;
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(kDtThreads, 1)
   uint64_t* res_full = drain + 1;            // [4 warps][kDtBufs]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(res_full + 4 * kDtBufs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  const int warp = warp_id(), lane = lane_id();
+  const int warp = warp_uniform(warp_id()), lane = lane_id();
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int tile0 = blockIdx.x / 2, step = gridDim.x / 2;
@@ -311,52 +316,65 @@ __global__ void __launch_bounds__(kDtThreads, 1)
   const uint32_t tmem = *tmem_holder;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int tile = tile0; ok && tile < p.tiles; tile += step) {
-        int tn, tm;
-        dense_tile_at(p, tile, tn, tm);
-        const int f0 = tn * 256 + (int)rank * 128, t0 = tm * p.bt + (int)rank * half;
-        for (int kb = 0; kb < KB; ++kb, ++it) {
-          const int st = it % kDtStages;
-          if (!mbar_wait(&empty[st], ((it / kDtStages) & 1) ^ 1, abort_flag, kDevErrTmaEmpty)) { ok = false; break; }
-          if (leader) mbar_arrive_expect_tx(&full[st], 2 * (128 * 128 + x_bytes));
-          const uint32_t bar = mapa_shared(&full[st], 0);
+    const bool issue = elect_one();
+    const uint32_t full0 = mapa_shared(full, 0);   // the leader's barriers
+    const uint32_t tx = 2 * (128 * 128 + x_bytes);
+    int it = 0;
+    bool ok = true;
+    for (int tile = tile0, st = 0, par = 1; ok && tile < p.tiles; tile += step) {
+      int tn, tm;
+      dense_tile_at(p, tile, tn, tm);
+      const int f0 = tn * 256 + (int)rank * 128, t0 = tm * p.bt + (int)rank * half;
+      for (int kb = 0; kb < KB; ++kb, ++it) {
+        if (!mbar_wait_warp(&empty[st], par, abort_flag, kDevErrTmaEmpty)) { ok = false; break; }
+        if (issue) {
+          if (leader) mbar_arrive_expect_tx(&full[st], tx);
           uint8_t* base = smem + st * kDtStageBytes;
-          tma_load_2d_pair(base, &tmap_w, bar, kb * 64, f0);
-          tma_load_2d_pair(base + 128 * 128, &tmap_x, bar, kb * 64, t0);
+          tma_load_2d_pair(base, &tmap_w, full0 + st * 8, kb * 64, f0);
+          tma_load_2d_pair(base + 128 * 128, &tmap_x, full0 + st * 8, kb * 64, t0);
         }
+        if (++st == kDtStages) { st = 0; par ^= 1; }
       }
-      // our copies signal the leader's barrier: wait until the pair's MMAs have released the stages
-      // we filled, then every copy has landed
+    }
+    // our copies signal the leader's barrier: wait until the pair's MMAs have released the stages
+    // we filled, then every copy has landed
+    if (issue)
       for (int i = it > kDtStages ? it - kDtStages : 0; i < it; ++i)
         mbar_drain(&empty[i % kDtStages], (i / kDtStages) & 1);
-    }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {   // the whole warp runs with uniform values, one elected thread issues
       const uint32_t idesc = make_idesc_f16(BF16, 256, p.bt);
-      int it = 0, n = 0;
+      const uint32_t tb = warp_uniform(tmem);
+      const uint64_t desc = smem_desc_kmajor_sw128(smem_u32(smem));   // counts in units of 16 bytes
+      const bool issue = elect_one();
+      int n = 0;
       bool ok = true;
-      for (int tile = tile0; ok && tile < p.tiles; tile += step, ++n) {
+      for (int tile = tile0, st = 0, par = 0; ok && tile < p.tiles; tile += step, ++n) {
         const int a = n & 1;
-        if (!mbar_wait_cluster_ns(&acc_empty[a], ((n >> 1) & 1) ^ 1, kDevErrAccEmpty, OC_WAIT_NS)) { *abort_flag = 1; break; }
-        tc_fence_after();
-        for (int kb = 0; kb < KB; ++kb, ++it) {
-          const int st = it % kDtStages;
-          if (!mbar_wait(&full[st], (it / kDtStages) & 1, abort_flag, kDevErrTmaFull)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t wa = smem_u32(smem + st * kDtStageBytes), xa = wa + 128 * 128;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            tc_mma_ss_pair(tmem + a * 256, smem_desc_kmajor_sw128(wa + j * 32), smem_desc_kmajor_sw128(xa + j * 32),
-                           idesc, (kb | j) != 0 ? 1u : 0u);
-          tc_commit_pair(&empty[st], 0x3);
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster_ns(&acc_empty[a], ((n >> 1) & 1) ^ 1, kDevErrAccEmpty, OC_WAIT_NS))) {
+          *abort_flag = 1;
+          break;
         }
-        if (ok) tc_commit_pair(&acc_full[a], 0x3);
+        tc_fence_after();
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!mbar_wait_warp(&full[st], par, abort_flag, kDevErrTmaFull)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t wd = desc + st * (kDtStageBytes / 16), xd = wd + 128 * 128 / 16;
+          if (issue) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tc_mma_ss_pair(tb + a * 256, wd + j * 2, xd + j * 2, idesc, (kb | j) != 0 ? 1u : 0u);
+            tc_commit_pair(&empty[st], 0x3);
+          }
+          if (++st == kDtStages) { st = 0; par ^= 1; }
+        }
+        if (ok && issue) tc_commit_pair(&acc_full[a], 0x3);
       }
-      tc_commit_pair(drain, 0x1);
-      mbar_drain(drain, 0);
+      if (issue) {
+        tc_commit_pair(drain, 0x1);
+        mbar_drain(drain, 0);
+      }
+      __syncwarp();
     }
   } else if (warp >= 4) {
     const int q4 = warp & 3;
