@@ -148,10 +148,26 @@ int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, o
   return launch_check("dense_gemm");
 }
 
-// Equal token tiles, a multiple of 32 tokens, at most 256.
-int dense_bt(int M) {
-  const int tiles = (M + 255) / 256;
-  return ((M + tiles - 1) / tiles + 31) / 32 * 32;
+// Tokens of a tile for the pair kernel: equal tiles of a multiple of 32 tokens, the size with the least
+// (waves of CTA pairs) x (time of one tile). A 64-k step of a tile takes about 2.3 cycles per token
+// (measured 590 at 256 tokens, 295 at 128), but no less than about 250, where the weights' stream bounds
+// it; a wave costs about 2500 cycles besides. Measured on 256 x 4096 x 4096: tiles of 256, 128, 64, 32 tokens
+// take 25.1, 18.3, 17.5 and 24.0 us; on 256 x 12288 x 4096: 28.7, 35.6, 42.1 and 55.0 us.
+int dense_bt(int M, int tiles_n, int K, int pairs) {
+  const int kb = (K + 63) / 64;
+  int best = 256;
+  double best_cost = 1e300;
+  for (int want = 256; want >= 32; want -= 32) {
+    const int tiles_m = (M + want - 1) / want;
+    const int bt = ((M + tiles_m - 1) / tiles_m + 31) / 32 * 32;
+    const double waves = std::ceil((double)tiles_n * tiles_m / pairs);
+    const double cost = waves * (kb * std::max(250.0, 2.3 * bt) + 2500.0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = bt;
+    }
+  }
+  return best;
 }
 
 template <bool BF16, int ACT, bool RES>
@@ -160,8 +176,9 @@ int launch_dense_tile(const void* x, int64_t ldx, const void* w, int64_t ldw, co
   const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   oc::DenseTileParams p{};
   p.d = d;
-  p.bt = dense_bt(d.M);
+  const int max_pairs = sm_count(dev) / 2;
   p.tiles_n = (d.N + 255) / 256;
+  p.bt = dense_bt(d.M, p.tiles_n, d.K, max_pairs);
   p.tiles_m = (d.M + p.bt - 1) / p.bt;
   const long long tiles = (long long)p.tiles_n * p.tiles_m;
   if (tiles > INT_MAX / 2) return fail(OC_ERR_INVALID, "dense_gemm: %lld tiles", tiles);
@@ -179,7 +196,7 @@ int launch_dense_tile(const void* x, int64_t ldx, const void* w, int64_t ldw, co
   }
   auto kern = oc::dense_tile_kernel<BF16, ACT, RES>;
   if (int rc = set_smem(kern, oc::kDtSmem)) return rc;
-  const int pairs = (int)std::min<long long>(tiles, sm_count(dev) / 2);
+  const int pairs = (int)std::min<long long>(tiles, max_pairs);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
   cfg.blockDim = dim3(oc::kDtThreads);
@@ -210,10 +227,16 @@ int launch_dense_tile_act(const void* x, int64_t ldx, const void* w, int64_t ldw
 template <bool BF16>
 int launch_dense(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& p, int dev,
                  cudaStream_t stream) {
+  // The K-splitting kernel up to 32 tokens, where streaming the weights through every SM decides (one token,
+  // weights from HBM, 4096 x 4096: 12.8 us against 16.8 of the pairs; 1024 x 8192: 10.8 against 27.1). Above, the
+  // pairs (64 tokens, 2560 x 2560: 13.9 against 11.8), unless few of them would walk a long K (64 tokens,
+  // 1024 x 8192: 13.8 against 26.9; 128 tokens: 16.2 against 25.1).
+  const int least_tiles = (p.N + 255) / 256 * ((p.M + 31) / 32);   // of the pairs, at their smallest size
   if (p.M <= 16) return launch_dense_split<BF16, 16>(x, ldx, w, ldw, p, dev, stream);
   if (p.M <= 32) return launch_dense_split<BF16, 32>(x, ldx, w, ldw, p, dev, stream);
-  if (p.M <= 64) return launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream);
-  if (p.M <= 128) return launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
+  if (p.M <= 128 && least_tiles <= 24 && p.K > 4096)
+    return p.M <= 64 ? launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream)
+                     : launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
   return p.residual ? launch_dense_tile_act<BF16, true>(x, ldx, w, ldw, p, dev, stream)
                     : launch_dense_tile_act<BF16, false>(x, ldx, w, ldw, p, dev, stream);
 }

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kDsThreads)
 // 256 features x up to 256 tokens with cta_group::2 MMAs: each CTA holds its 128 features' weights and
 // half of the tokens' activations, so an SM moves 32 KB of shared memory per 128 x 256 x 64 product instead
 // of 48 KB. Features are the MMA's M and tokens its N: a ragged token count is split into equal tiles
-// of a multiple of 32 tokens (517 tokens: three of 192 instead of three of 256). The accumulator is double
+// of a multiple of 32 tokens. The accumulator is double
 // buffered in TMEM, so four epilogue warps drain a tile while the next one is multiplied. Every epilogue
 // warp owns 32 features (its TMEM lanes) and moves [32 tokens x 32 features] pieces through its own four
 // buffers by TMA, residual pieces loaded two ahead; outputs or residuals that a tensor map cannot

@@ -362,6 +362,20 @@ def test_linear_sizes(cuda_device, M, dims):
     assert error_word(dev) == 0
 
 
+@pytest.mark.parametrize("shape", [(33, 1000, 8192), (64, 520, 6000), (100, 264, 5120), (128, 1024, 4104), (65, 6400, 4160),
+                                   (200, 4100, 1024), (517, 2056, 640), (1030, 300, 72), (2049, 1288, 128)])
+def test_linear_kernel_choice(cuda_device, shape):
+    """Both kernels around the border of their rule (few tokens and a long K), and every token tile size."""
+    from onecomp_runtime.layers import linear_fused
+    dev = cuda_device
+    M, N, K = shape
+    x, w, b, r = randn(dev, M, K, seed=1), randn(dev, N, K, seed=2, std=K ** -0.5), randn(dev, N, seed=3), \
+        randn(dev, M, N, seed=4)
+    with torch.no_grad():
+        ref.check(linear_fused(x, w, b, activation="gelu", residual=r), *ref.linear(x, w, b, "gelu", r), f"{shape}")
+    assert error_word(dev) == 0
+
+
 @pytest.mark.parametrize("act", [None, "gelu_tanh", "gelu", "silu", "relu"])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("M", [3, 300])
