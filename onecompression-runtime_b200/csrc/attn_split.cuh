@@ -4,9 +4,10 @@
 // into tiles of 16 rows, so a group of query heads shares every key it reads. The work of a call is
 // the list of 64-key blocks of all (sequence, key head, row tile) items in order; the CTAs of one
 // full wave take equal runs of that list, found on the device from the length tables, so ragged
-// lengths and long caches spread over every SM without the host knowing a length. Inside a run
-// four warps take 16-key slices in turn, each through a private cp.async ring (no CTA barrier while
-// streaming), with m16n8k16 tensor-core products, the running row maximum and sum in fp32 and base 2
+// lengths and long caches spread over every SM without the host knowing a length. Inside a run four
+// or eight warps take 16-key slices in turn, each through a private cp.async ring of K and V units (no
+// CTA barrier while streaming; TMA boxes of 16 keys, issued by the warps or by a warp of their own, took
+// 146 and 176 us where these copies take 137: 48 tokens over caches up to 8192), with m16n8k16 tensor-core products, the running row maximum and sum in fp32 and base 2
 // exponents. The warps are joined through shared memory; an item that spans CTAs leaves fp32
 // partials (maximum, sum, unnormalized output) that attn_join_kernel adds in CTA order: no atomics,
 // the same bits on every run.
@@ -16,25 +17,27 @@
 
 namespace oc {
 
-constexpr int kSplitWarps = 4;
-constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kSplitRows = 16;      // rows of a tile
 constexpr int kSplitBlock = 64;     // keys of a work unit
 constexpr int kSplitDescInts = 8;
 
 template <int DP> struct SplitCfg {
-  static constexpr int kKvBytes = 16 * DP * 2;                 // 16 keys (or values)
-  static constexpr int kStageBytes = 2 * kKvBytes;
-  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kWarps = DP == 256 ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kUnitBytes = 16 * DP * 2;               // 16 keys, or their values
+  static constexpr int kUnits = DP == 256 ? 3 : DP == 128 ? 6 : 12;   // of a warp's ring: K, V, K, V, ...
   static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
-  static constexpr int kRingBytes = kSplitWarps * kStages * kStageBytes;   // 96 KB; 192 KB at DP = 256
+  static constexpr int kRingBytes = kWarps * kUnits * kUnitBytes;   // 96 KB; 192 KB at DP = 256
   static constexpr int kPitch = DP + 8;                        // floats of a joined row
   static constexpr int kPartFloats = kSplitRows * (DP + 2);    // one partial: O [16][DP], m [16], l [16]
-  static_assert(kSplitWarps * kSplitRows * kPitch * 4 <= kRingBytes, "the warps' outputs fit the ring");
+  static_assert(kWarps * kSplitRows * kPitch * 4 <= kRingBytes, "the warps' outputs fit the ring");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -72,10 +75,11 @@ __device__ __forceinline__ long long split_units(const AttnParams& p, const Seq&
 }
 
 template <bool BF16, int DP>
-__global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_split_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPerSm) attn_split_kernel(const AttnParams p) {
   using Cfg = SplitCfg<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sm_m[kSplitWarps][kSplitRows], sm_l[kSplitWarps][kSplitRows];
+  constexpr int kWarps = Cfg::kWarps;
+  __shared__ float sm_m[kWarps][kSplitRows], sm_l[kWarps][kSplitRows];
   __shared__ int sm_odd;   // an infinity or NaN was taken out of the item's values
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = warp_id(), lane = lane_id();
@@ -87,25 +91,31 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
   }
   __syncthreads();
 
-  // the call's units, then this CTA's run of them (every warp finds it for itself)
-  long long total = 0;
+  // the call's units, then this CTA's run of them (every warp finds it for itself; with up to 32
+  // sequences the tables are read once)
+  long long total = 0, mine = 0;
   for (int base = 0; base < p.B; base += 32) {
-    long long u = 0;
-    if (base + lane < p.B) u = split_units(p, attn_seq(p, base + lane, blockIdx.x == 0 && warp == 0));
+    mine = base + lane < p.B ? split_units(p, attn_seq(p, base + lane, blockIdx.x == 0 && warp == 0)) : 0;
+    long long sum = mine;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    total += u;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    total += sum;
   }
   if (p.zero_tail) attn_zero_tail(p, blockIdx.x, gridDim.x);
-  const long long n = total < (long long)gridDim.x ? total : (long long)gridDim.x;
-  if (blockIdx.x >= n) return;
-  const long long u_end = total * (blockIdx.x + 1) / n;
-  long long u = total * blockIdx.x / n;
+  const int n = (int)min(total, (long long)gridDim.x);   // CTAs with work
+  if ((int)blockIdx.x >= n) return;
+  long long u, u_end;
+  if (total < (1ll << 22)) {   // the grid is below 2^10: 32-bit divisions
+    u = (unsigned)total * blockIdx.x / (unsigned)n;
+    u_end = (unsigned)total * (blockIdx.x + 1) / (unsigned)n;
+  } else {
+    u = total * blockIdx.x / n;
+    u_end = total * (blockIdx.x + 1) / n;
+  }
   int b = 0;
   long long seq_begin = 0;   // first unit of sequence b
   for (int base = 0; base < p.B; base += 32) {
-    long long mine = 0;
-    if (base + lane < p.B) mine = split_units(p, attn_seq(p, base + lane));
+    if (p.B > 32) mine = base + lane < p.B ? split_units(p, attn_seq(p, base + lane)) : 0;
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -123,7 +133,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
   }
   Seq s = attn_seq(p, b);
 
-  uint8_t* ring = smem + warp * (Cfg::kStages * Cfg::kStageBytes);
+  uint8_t* ring = smem + warp * (Cfg::kUnits * Cfg::kUnitBytes);
   const uint32_t ring_addr = smem_u32(ring);
   constexpr int kCh = DP / 8;                      // 16-byte chunks of a row
   constexpr int kIter = 16 * kCh / 32;             // chunks per lane of one 16-row matrix
@@ -136,11 +146,11 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     }
     const int nblk = split_blocks(s.nk);
     const long long rel = u - seq_begin;
-    const long long item = rel / nblk;
+    const long long item = rel < (1ll << 31) ? (long long)((unsigned)rel / (unsigned)nblk) : rel / nblk;
     const int blk0 = (int)(rel - item * nblk);
     const int blk1 = (int)min((long long)nblk, blk0 + (u_end - u));
     const long long tiles = split_tiles(p, s.nq);
-    const int kvh = (int)(item / tiles);
+    const int kvh = (item | tiles) < (1ll << 31) ? (int)((unsigned)item / (unsigned)tiles) : (int)(item / tiles);
     const long long row0 = (item - kvh * tiles) * kSplitRows;
     const int rows = (int)min((long long)kSplitRows, (long long)s.nq * p.G - row0);
     const int kbeg = blk0 * kSplitBlock, kend = min(s.nk, blk1 * kSplitBlock);
@@ -159,26 +169,35 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     const bool c_in = c_ch * 8 < p.D;
     const uint16_t* k_src = kb + (long long)(kbeg + c_row) * p.k_st + c_ch * 8;
     const uint16_t* v_src = vb + (long long)(kbeg + c_row) * p.v_st + c_ch * 8;
-    auto issue = [&](int sl, int stage) {
-      if (sl < slices) {
-        const uint16_t* ks = k_src + (long long)sl * 16 * p.k_st;
-        const uint16_t* vs = v_src + (long long)sl * 16 * p.v_st;
-        const uint32_t dst = ring_addr + stage * Cfg::kStageBytes + c_row * (DP * 2);
+    // the warp's unit n of this item: K (even) or V (odd) of its slice n / 2, into ring place `at`
+    const int units = (slices > warp ? (slices - warp + kWarps - 1) / kWarps : 0) * 2;
+    auto issue = [&](int n, int at) {
+      if (n < units) {
+        const int sl = warp + (n >> 1) * kWarps;
+        const long long st = n & 1 ? p.v_st : p.k_st;
+        const uint16_t* src = (n & 1 ? v_src : k_src) + (long long)sl * 16 * st;
+        const uint32_t dst = ring_addr + at * Cfg::kUnitBytes + c_row * (DP * 2);
         const int left = kend - kbeg - sl * 16 - c_row;   // rows this lane may still copy
+        if (sl * 16 + 16 <= kend - kbeg && p.D == DP) {
 #pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-          const bool ok = c_in && i * kStep < left;
-          const uint32_t off = dst + i * kStep * (DP * 2) + ((c_ch ^ ((i * kStep + c_row) & 7)) * 16);
-          cp_async16(off, ok ? ks : p.k, ok);
-          cp_async16(off + Cfg::kKvBytes, ok ? vs : p.v, ok);
-          ks += kStep * p.k_st;
-          vs += kStep * p.v_st;
+          for (int i = 0; i < kIter; ++i) {
+            cp_async16(dst + i * kStep * (DP * 2) + ((c_ch ^ ((i * kStep + c_row) & 7)) * 16), src);
+            src += kStep * st;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kIter; ++i) {
+            const bool ok = c_in && i * kStep < left;
+            cp_async16(dst + i * kStep * (DP * 2) + ((c_ch ^ ((i * kStep + c_row) & 7)) * 16), ok ? src : p.k, ok);
+            src += kStep * st;
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    constexpr int NU = Cfg::kUnits;
 #pragma unroll 1
-    for (int i = 0; i < Cfg::kStages - 1; ++i) issue(warp + i * kSplitWarps, i);
+    for (int i = 0; i < NU - 1; ++i) issue(i, i);
 
     // this lane's two rows: last visible key, and the queries as A fragments
     int limit[2];
@@ -202,23 +221,34 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     const int first_limit = p.causal ? (int)(row0 / p.G) + s.nk - s.nq : kend - 1;   // of the tile's first token
     const int edge_begin = kbeg + max(0, min(first_limit + 1, kend) - kbeg) / 16 * 16;
     const bool has_edge = first_limit < kend - 1;
-    int stage = 0;
-    for (int sl = warp; sl < slices; sl += kSplitWarps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 2) : "memory");
-      __syncwarp();   // every lane's copies of this stage have landed; the stage refilled next is read
-      issue(sl + (Cfg::kStages - 1) * kSplitWarps, stage == 0 ? Cfg::kStages - 1 : stage - 1);
-      const uint32_t ks_addr = ring_addr + stage * Cfg::kStageBytes;
-      const uint32_t vs_addr = ks_addr + Cfg::kKvBytes;
+    // ldmatrix addresses: 16-byte chunk c of a row lies at ((c ^ (row & 7)) * 16) of its 128-byte part, so step k of
+    // a part's four flips bits of the lane's first address
+    const int k_row = (lane & 7) + ((lane >> 4) << 3), v_row = lane & 15;
+    const uint32_t k_at = ring_addr + k_row * (DP * 2) + ((((lane >> 3) & 1) ^ (k_row & 7)) << 4);
+    const uint32_t v_at = ring_addr + v_row * (DP * 2) + (((lane >> 4) ^ (v_row & 7)) << 4);
+    int place = 0;   // of the next unit to read; the one before it is refilled
+    auto step = [&](int n) {   // unit n has landed, and the unit that was read last makes room
+      asm volatile("cp.async.wait_group %0;" ::"n"(NU - 2) : "memory");
+      __syncwarp();
+      issue(n + NU - 1, place == 0 ? NU - 1 : place - 1);
+      const int at = place;
+      place = place + 1 == NU ? 0 : place + 1;
+      return at;
+    };
+    for (int n = 0; n < units; n += 2) {
+      const int sl = warp + (n >> 1) * kWarps;
+      const uint32_t ks_addr = k_at + step(n) * Cfg::kUnitBytes;
       const int key0 = kbeg + sl * 16;
-      float c[2][4] = {};
+      float c[2][4] = {}, c2[2][4] = {};   // two chains each: the products of one sum wait for one another
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         uint32_t r[4];
-        const int row = (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
-        ldsm_x4(ks_addr + row * (DP * 2) + ((ch ^ (row & 7)) * 16), r);
-        mma16816<BF16>(c[0], qa[ks], r[0], r[1]);
-        mma16816<BF16>(c[1], qa[ks], r[2], r[3]);
+        ldsm_x4((ks_addr ^ ((ks & 3) << 5)) + (ks >> 2) * 128, r);
+        mma16816<BF16>(ks & 1 ? c2[0] : c[0], qa[ks], r[0], r[1]);
+        mma16816<BF16>(ks & 1 ? c2[1] : c[1], qa[ks], r[2], r[3]);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { c[0][i] += c2[0][i]; c[1][i] += c2[1][i]; }
       // The exponents' reference follows the running maximum only when it grew by more than 2^8 (weights
       // up to 256 are as exact in 16 bits as weights up to 1): the output is rarely scaled.
       float top[2];
@@ -265,8 +295,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
       }
       // A value that a row does not see may be infinite or NaN, and its weight of zero must not turn that
       // into NaN: such values leave the slice, and the rows that see them add them at the end.
+      const int v_place = step(n + 1);
+      const uint32_t vs_addr = v_at + v_place * Cfg::kUnitBytes;
       if (has_edge && key0 >= edge_begin) {
-        uint4* vsl = reinterpret_cast<uint4*>(ring + stage * Cfg::kStageBytes + Cfg::kKvBytes);
+        uint4* vsl = reinterpret_cast<uint4*>(ring + v_place * Cfg::kUnitBytes);
 #pragma unroll 1
         for (int i = lane; i < 16 * kCh; i += 32) {
           uint4 x = vsl[i];
@@ -280,12 +312,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
 #pragma unroll
       for (int d2 = 0; d2 < DP / 16; ++d2) {
         uint32_t r[4];
-        const int row = lane & 15, ch = d2 * 2 + (lane >> 4);
-        ldsm_x4_trans(vs_addr + row * (DP * 2) + ((ch ^ (row & 7)) * 16), r);
+        ldsm_x4_trans((vs_addr ^ ((d2 & 3) << 5)) + (d2 >> 2) * 128, r);
         mma16816<BF16>(o[2 * d2], pa, r[0], r[1]);
         mma16816<BF16>(o[2 * d2 + 1], pa, r[2], r[3]);
       }
-      stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();   // the rings are read; they now hold the warps' outputs
@@ -307,16 +337,16 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
     __syncthreads();
     const bool whole = blk0 == 0 && blk1 == nblk;
     float* part = p.part + ((long long)blockIdx.x * 2 + (blk0 == 0 ? 1 : 0)) * Cfg::kPartFloats;
-    for (int i = threadIdx.x; i < rows * (DP / 4); i += kSplitThreads) {
+    for (int i = threadIdx.x; i < rows * (DP / 4); i += Cfg::kThreads) {
       const int r = i / (DP / 4), c4 = (i % (DP / 4)) * 4;
       float mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
       const float ref = mx == -INFINITY ? 0.f : mx;
       float lsum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float a = ex2(sm_m[w][r] - ref);
         const float4 x = *reinterpret_cast<const float4*>(osm + (w * kSplitRows + r) * Cfg::kPitch + c4);
         lsum += a * sm_l[w][r];
@@ -363,41 +393,85 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<DP>::kCtasPerSm) attn_
 }
 
 // Joins the partials of the item that CTA blockIdx.x began: slot 1 of that CTA, slot 0 of the CTAs
-// after it up to the item's last one, in that order. One warp per row.
+// after it up to the item's last one. Four rows to a block, four warps to a row, each of which takes
+// every fourth partial in order: eight independent loads are in flight, and the sums' order is fixed.
+constexpr int kJoinThreads = 512;
 template <bool BF16, int DP>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParams p) {
   using Cfg = SplitCfg<DP>;
+  constexpr int kV = DP / 32;   // columns of a lane
+  __shared__ float sm_acc[4][4][DP], sm_m[4][4], sm_l[4][4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int* desc = p.desc + blockIdx.x * kSplitDescInts;
-  const int r = blockIdx.y * 4 + warp_id(), lane = lane_id();
-  if (r >= desc[0]) return;
-  const int c0 = blockIdx.x, c1 = desc[1];
-  auto slot = [&](int c) { return p.part + ((long long)c * 2 + (c == c0 ? 1 : 0)) * Cfg::kPartFloats; };
-  float mx = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, slot(c)[kSplitRows * DP + r]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float lsum = 0.f;
-  constexpr int kV = DP / 32;   // columns of a lane
-  float acc[kV];
+  if ((int)blockIdx.y * 4 >= desc[0]) return;
+  const int row_in = warp_id() >> 2, part = warp_id() & 3, lane = lane_id();
+  const int r = blockIdx.y * 4 + row_in;
+  const int c0 = blockIdx.x, count = desc[1] - c0 + 1;
+  auto slot = [&](int i) { return p.part + ((long long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * Cfg::kPartFloats; };
+  float mx = -INFINITY, lsum = 0.f, acc[kV];
 #pragma unroll
   for (int i = 0; i < kV; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float* s = slot(c);
-    const float a = ex2(s[kSplitRows * DP + r] - ref);
-    lsum += a * s[kSplitRows * DP + kSplitRows + r];
+  // this warp's partials: part, part + 4, ...; a lane looks at one of up to 32 of them at a time
+  const int mine = count > part ? (count - part + 3) / 4 : 0;
+  for (int base = 0; base < mine; base += 32) {
+    float m = -INFINITY, l = 0.f;
+    if (base + lane < mine) {
+      const float* ml = slot(part + 4 * (base + lane)) + kSplitRows * DP + r;
+      m = ml[0];
+      l = ml[kSplitRows];
+    }
+    float top = fmaxf(mx, m);
 #pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] += a * s[r * DP + lane * kV + i];
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float old = ex2(mx - ref), w = ex2(m - ref);
+    mx = top;
+    float sum = w * l;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    lsum = lsum * old + sum;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] *= old;
+    const int here = min(32, mine - base);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float a = __shfl_sync(0xffffffffu, w, i);
+      const float* src = slot(part + 4 * (base + i)) + r * DP + lane * kV;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc[e] += a * src[e];
+    }
   }
-  const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+#pragma unroll
+  for (int e = 0; e < kV; ++e) sm_acc[row_in][part][lane * kV + e] = acc[e];
+  if (lane == 0) {
+    sm_m[row_in][part] = mx;
+    sm_l[row_in][part] = lsum;
+  }
+  __syncthreads();
+  if (part != 0 || r >= desc[0]) return;
+  float top = -INFINITY, total = 0.f, f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = fmaxf(top, sm_m[row_in][i]);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = ex2(sm_m[row_in][i] - ref);
+    total += f[i] * sm_l[row_in][i];
+  }
+  const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
   const long long row = *reinterpret_cast<const long long*>(desc + 4) + r;
   uint16_t* dst = p.out + (desc[2] + row / p.G) * p.o_st + (desc[3] * p.G + row % p.G) * p.o_sh + lane * kV;
   if (lane * kV < p.D) {
 #pragma unroll
-    for (int i = 0; i < kV; i += 2)
-      *reinterpret_cast<uint32_t*>(dst + i) = pack2_rn<BF16>(acc[i] * inv, acc[i + 1] * inv);
+    for (int e = 0; e < kV; e += 2) {
+      float x[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[0] += f[i] * sm_acc[row_in][i][lane * kV + e];
+        x[1] += f[i] * sm_acc[row_in][i][lane * kV + e + 1];
+      }
+      *reinterpret_cast<uint32_t*>(dst + e) = pack2_rn<BF16>(x[0] * inv, x[1] * inv);
+    }
   }
 }
 

@@ -54,6 +54,7 @@ template <int DP> struct TileCfg {
                                                             // where loads follow the products unit by unit
   static constexpr int kGroups = kUnits / kGroup;
   static constexpr int kSoftmaxThreads = kTiles * 128;
+  static constexpr int kSoftmaxRegs = 216, kAuxRegs = 72;   // of two tiles: 168 at launch for each of 384 threads
   static constexpr int kThreads = kSoftmaxThreads + 128;
   static constexpr int kQBytes = kTiles * kUnits * kTileUnitBytes;
   static constexpr int kRingBytes = kSlots * kUnits * kTileUnitBytes;
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   const uint32_t tmem = *tmem_holder;
 
   if (warp >= kAux) {
-    if constexpr (kTwo) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (kTwo) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kAuxRegs));
     if (warp == kAux) {
       // ------------------------------------------------------------ TMA
       if (lane == 0) {
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax: one thread per row
-    if constexpr (kTwo) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (kTwo) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
     const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = w.r0 + t * 128 + (warp & 3) * 32 + lane;

@@ -32,6 +32,17 @@ template <typename K> int set_smem(K kern, int bytes) {
                     "shared memory limit");
 }
 
+// A kernel that moves registers between its warpgroups (setmaxnreg) waits for ever if the launch gives it
+// fewer than the shares add up to, so the compiled count is checked before the first launch.
+template <typename K> int check_registers(K kern, int threads, int needed, const char* what) {
+  cudaFuncAttributes at;
+  if (int rc = cuda_check(cudaFuncGetAttributes(&at, kern), what)) return rc;
+  if (at.numRegs * threads < needed)
+    return fail(OC_ERR_UNSUPPORTED, "%s: built with %d registers a thread, %d threads need %d in all", what, at.numRegs,
+                threads, needed);
+  return OC_OK;
+}
+
 // ------------------------------------------------------------------ rotary positions
 template <int DT, int V, bool INTER>
 int launch_rope(const oc::RopeParams& p0, int sms, cudaStream_t stream) {
@@ -75,9 +86,10 @@ size_t split_ws_bytes(int dp, int ctas) {
 template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas, cudaStream_t stream) {
   auto kern = oc::attn_split_kernel<BF16, DP>;
   if (int rc = set_smem(kern, oc::SplitCfg<DP>::kRingBytes)) return rc;
-  kern<<<ctas, oc::kSplitThreads, oc::SplitCfg<DP>::kRingBytes, stream>>>(p);
+  kern<<<ctas, oc::SplitCfg<DP>::kThreads, oc::SplitCfg<DP>::kRingBytes, stream>>>(p);
   if (int rc = launch_check("attention (split)")) return rc;
-  return launch_pdl(oc::attn_join_kernel<BF16, DP>, dim3((unsigned)ctas, oc::kSplitRows / 4), dim3(128), 0, stream,
+  return launch_pdl(oc::attn_join_kernel<BF16, DP>, dim3((unsigned)ctas, oc::kSplitRows / 4), dim3(oc::kJoinThreads), 0,
+                    stream,
                     "attention (join)", p);
 }
 
@@ -110,6 +122,10 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, cudaStream_t stre
   const int negate = p.scale_log2 < 0.f;
   p.scale_log2 = std::fmax(std::fabs(p.scale_log2), 1e-30f);
   auto kern = oc::attn_tile_kernel<BF16, DP>;
+  static const int regs_rc = check_registers(
+      kern, Cfg::kThreads, Cfg::kTiles == 2 ? Cfg::kSoftmaxThreads * Cfg::kSoftmaxRegs + 128 * Cfg::kAuxRegs : 0,
+      "attention (tile)");
+  if (regs_rc) return fail(regs_rc, "attention (tile): register count of the build");
   if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
   kern<<<slots * p.Hq, Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, slots, negate);
   return launch_check("attention (tile)");
