@@ -60,6 +60,21 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     return freq, gain
 
 
+_NO_TENSOR = (None, 0, 0, None, 0, 0, 0)
+
+
+def _out_of_place(t: torch.Tensor, T: int, D: int, dtype: torch.dtype, dev: torch.device):
+    """(what the kernel reads, the new output, kernel arguments) for ``t`` [..., H, D]."""
+    out = torch.empty(t.shape, dtype=dtype, device=dev)
+    src = t if t.dim() == 3 else t.reshape(T, -1, D) if t.numel() else t.reshape(T, t.shape[-2], D)
+    st, sh, sd = src.stride()
+    if sd != 1 and D > 1:
+        src = src.contiguous()
+        st, sh, sd = src.stride()
+    H = src.shape[1]
+    return src, out, (src.data_ptr(), st, sh, out.data_ptr(), H * D, D, H)
+
+
 def _in_place(what: str, t: torch.Tensor, T: int) -> tuple:
     """Kernel arguments that rotate ``t`` [..., H, D] where it lies."""
     H, D = t.shape[-2:]
@@ -124,6 +139,7 @@ class RotaryEmbedding(torch.nn.Module):
         elif inv_freq is None:
             freq, gain = rotary_frequencies(R, base, scaling)
         self.inv_freq, self.gain = freq, float(gain)
+        self._interleaved = layout == "interleaved"
         # fraction of a turn per position as 0.64 fixed point (two's complement bits in int64)
         turns = [int(round(math.fmod(f / (2.0 * math.pi), 1.0) * 2.0 ** 64)) % 2 ** 64 for f in freq]
         self._turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
@@ -148,50 +164,51 @@ class RotaryEmbedding(torch.nn.Module):
         int64 [...], with ``axes`` [..., len(axes)]. Returns the rotated ``(q, k)``, rounded once; ``inplace``
         writes into the inputs (which may be slices of one projection's output)."""
         what = "RotaryEmbedding"
-        D = self.head_dim
-        lead = q.shape[:-2]
-        A = 1 if self.axes is None else len(self.axes)
-        want = lead if self.axes is None else (*lead, A)
-        for name, t in (("q", q), ("k", k)):
-            if t is not None and (t.dim() < 3 or t.shape[:-2] != lead or t.shape[-1] != D):
-                raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {(*lead, 'heads', D)}")
-        if positions.shape != want or positions.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{what}: positions {positions.dtype} {tuple(positions.shape)}, expected int32 or int64 "
-                             f"{tuple(want)}")
-        dtype = q.dtype
-        if dtype not in _lib.DT or (k is not None and k.dtype != dtype):
+        D, dtype = self.head_dim, q.dtype
+        q_shape, p_shape = q.shape, positions.shape
+        tokens, A = q_shape[:-2], 1
+        fits = q.dim() >= 3 and q_shape[-1] == D
+        if self.axes is None:
+            fits_p = p_shape == tokens
+        else:
+            A = len(self.axes)
+            fits_p = p_shape[:-1] == tokens and positions.dim() > 0 and p_shape[-1] == A
+        if not fits or (k is not None and (k.dim() != q.dim() or k.shape[-1] != D or k.shape[:-2] != tokens)):
+            raise ValueError(f"{what}: q {tuple(q_shape)}, k {None if k is None else tuple(k.shape)}, expected "
+                             f"{(*tokens, 'heads', D)}")
+        pos_dtype = positions.dtype
+        if not fits_p or (pos_dtype is not torch.int64 and pos_dtype is not torch.int32):
+            raise ValueError(f"{what}: positions {pos_dtype} {tuple(p_shape)}, expected int32 or int64 "
+                             f"{tuple(tokens) if self.axes is None else (*tokens, A)}")
+        if dtype not in _lib.DT or (k is not None and k.dtype is not dtype):
             raise TypeError(f"{what} takes fp16, bf16 or fp32 of one dtype, got {dtype} and "
                             f"{None if k is None else k.dtype}")
         inference_only(what, q, k)
         dev = one_device(what, q, k, positions)
-        T = lead[0] if len(lead) == 1 else math.prod(lead)
-        sides = []   # per tensor: result, what the kernel reads, its arguments
-        for t in (q, k):
-            if t is None:
-                sides.append((None, None, (None, 0, 0, None, 0, 0, 0)))
-            elif inplace:
-                sides.append((t, t, _in_place(what, t, T)))
-            else:
-                src = t if t.dim() == 3 else t.reshape(T, -1, D)
-                if src.stride(2) != 1:
-                    src = src.contiguous()
-                res = torch.empty(t.shape, dtype=dtype, device=dev)
-                H = src.shape[1]
-                sides.append((res, src, (src.data_ptr(), src.stride(0), src.stride(1), res.data_ptr(), H * D, D, H)))
+        T = q_shape[0] if len(tokens) == 1 else math.prod(tokens)
+        if inplace:
+            q_out, k_out = q, k
+            q_args = _in_place(what, q, T)
+            k_args = _NO_TENSOR if k is None else _in_place(what, k, T)
+        else:
+            q, q_out, q_args = _out_of_place(q, T, D, dtype, dev)
+            k_out, k_args = None, _NO_TENSOR
+            if k is not None:
+                k, k_out, k_args = _out_of_place(k, T, D, dtype, dev)
         if T == 0:
-            return sides[0][0], sides[1][0]
-        turns, axis = self._table(dev)
-        pos, pos_st = positions, 1
-        if positions.dim() != 1 or positions.stride(0) != 1:
-            pos = positions.reshape(T, A)
-            if A > 1 and pos.stride(1) != 1:
-                pos = pos.contiguous()
-            pos_st = pos.stride(0)
+            return q_out, k_out
+        turns, axis = self._tables.get(dev.index) or self._table(dev)
+        pos_st = 1
+        if A > 1 or positions.dim() != 1 or positions.stride(0) != 1:
+            positions = positions.reshape(T, A)
+            if A > 1 and positions.stride(1) != 1:
+                positions = positions.contiguous()
+            pos_st = positions.stride(0)
         with on_device(dev):
-            _lib.call("oc_b200_rope", *sides[0][2], *sides[1][2], _lib.DT[dtype], T, D, self.rotary_dim, pos.data_ptr(),
-                      pos.dtype == torch.int64, pos_st, turns.data_ptr(), _lib.ptr(axis), self.gain,
-                      self.layout == "interleaved", _lib.stream_of(dev))
-        return sides[0][0], sides[1][0]
+            _lib.call("oc_b200_rope", *q_args, *k_args, _lib.DT[dtype], T, D, self.rotary_dim, positions.data_ptr(),
+                      pos_dtype is torch.int64, pos_st, turns.data_ptr(), None if axis is None else axis.data_ptr(),
+                      self.gain, self._interleaved, _lib.stream_of(dev))
+        return q_out, k_out
 
     def extra_repr(self) -> str:
         return (f"head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, layout={self.layout}, axes={self.axes}, "
