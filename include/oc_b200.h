@@ -320,9 +320,9 @@ int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t
  * Query rows outside every sequence stay as they were, or become zeros with zero_tail (rows behind
  * cu_q[B]). The tables are read on the device; values outside the tensors are clamped and set the
  * device error word. max_q (0: unknown) is a hint of the longest query run; it only picks a kernel.
- * workspace: oc_b200_attention_workspace(D) bytes on the current device, any contents, 16-byte
- * aligned, not shared by calls that may run at once. out must not overlap the inputs. */
-size_t oc_b200_attention_workspace(int D);
+ * workspace: oc_b200_attention_workspace bytes for the same sizes on the current device (may be 0), any
+ * contents, 16-byte aligned, not shared by calls that may run at once. out must not overlap the inputs. */
+size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q);
 int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                       const void* v, int64_t v_st, int64_t v_sh, void* out, int64_t o_st, int64_t o_sh, int dtype,
                       int Tq, int Tk, int Hq, int Hkv, int D, const int32_t* cu_q, const int32_t* cu_k,

@@ -18,10 +18,12 @@
 //     of the sequence): rows behind the keys become zeros, and in causal blocks infinities and NaN,
 //     which a weight of zero must not turn into NaN, are taken out and added afterwards by the rows
 //     that see them.
-// Tiles are numbered without the host knowing a length: sequence b's tiles start at
-// floor(cu_q[b] / rows) + b, which leaves room for every sequence's ragged last tile; a CTA whose tile
-// lies behind its sequence's end exits. Every head's tiles run from its last row up, so that the long
-// causal tiles start first. All waits are bounded (common.cuh).
+// Tiles are numbered without the host knowing a length: sequence b's CTAs start at
+// floor(cu_q[b] / tokens) + b, which leaves room for every sequence's ragged last tile; a CTA whose tokens
+// lie behind its sequence's end exits. Every head's tiles run from its last token up, so that the long
+// causal tiles start first. Where the tiles of a call would leave SMs idle, several CTAs take a part of
+// the keys each and leave fp32 partials that attn_tile_join_kernel adds in order. All waits are bounded
+// (common.cuh).
 #pragma once
 
 #include <type_traits>
@@ -99,17 +101,24 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 
 struct TileMaps { CUtensorMap q, k, v; };
 
-// What a CTA works on; every role derives the same numbers.
-struct TileWork {
-  Seq s;
-  int head, kvh, r0, ntile, nblk, e0;   // e0: first block that some row of the CTA does not see whole
-  int nb[2];                            // blocks of each tile
+struct TileGrid {
+  int tokens;    // of a tile: 128 / G
+  int slots;     // CTAs' token ranges over all sequences, ragged ends included
+  int splits;    // CTAs that share the keys of a range
+  float* part;   // splits > 1: [slot, key head][split][tile][128 rows] O [DP], then m, l
 };
 
-template <int DP> __device__ __forceinline__ bool tile_work(const AttnParams& p, int n_slots, TileWork& w) {
-  constexpr int R = TileCfg<DP>::kRows;
-  w.head = blockIdx.x / n_slots;
-  const int slot = n_slots - 1 - blockIdx.x % n_slots;
+// What a CTA works on; every role derives the same numbers. With a split, the keys are those of its part:
+// the sequence's key rows then start at the part's first block.
+struct TileWork {
+  Seq s;
+  int kvh, t0, ntile, nblk, e0, split;   // t0: first token; e0: first block that some row does not see whole
+  int nb[2];                             // blocks of each tile
+};
+
+// The sequence and first token of a token range; false behind the sequence's end.
+template <int DP> __device__ __forceinline__ bool tile_range(const AttnParams& p, const TileGrid& tg, int slot, TileWork& w) {
+  const int R = TileCfg<DP>::kTiles * tg.tokens;
   int lo = 0, hi = p.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -117,20 +126,32 @@ template <int DP> __device__ __forceinline__ bool tile_work(const AttnParams& p,
     if (q0 / R + mid <= slot) lo = mid; else hi = mid;
   }
   w.s = attn_seq(p, lo);
-  const long long r0 = (long long)(slot - (w.s.q0 / R + lo)) * R;
-  if (r0 < 0 || r0 >= w.s.nq) return false;
-  w.r0 = (int)r0;
-  w.kvh = w.head / p.G;
-  w.ntile = min(TileCfg<DP>::kTiles, (w.s.nq - w.r0 + 127) / 128);
+  const long long t0 = (long long)(slot - (w.s.q0 / R + lo)) * R;
+  if (t0 < 0 || t0 >= w.s.nq) return false;
+  w.t0 = (int)t0;
+  w.ntile = min(TileCfg<DP>::kTiles, (w.s.nq - w.t0 + tg.tokens - 1) / tg.tokens);
+  return true;
+}
+
+template <int DP> __device__ __forceinline__ bool tile_work(const AttnParams& p, const TileGrid& tg, TileWork& w) {
+  const int unit = blockIdx.x / tg.splits;
+  w.split = blockIdx.x - unit * tg.splits;
+  w.kvh = unit / tg.slots;
+  if (!tile_range<DP>(p, tg, tg.slots - 1 - (unit - w.kvh * tg.slots), w)) return false;
   const int off = w.s.nk - w.s.nq;
-  for (int t = 0; t < 2; ++t) {
-    const int last = min(w.s.nq, w.r0 + (t + 1) * 128) - 1;
+  auto blocks = [&](int t) {   // that the tile's last token sees
+    const int last = min(w.s.nq, w.t0 + (t + 1) * tg.tokens) - 1;
     const int keys = p.causal ? min(w.s.nk, max(0, last + off + 1)) : w.s.nk;
-    w.nb[t] = t < w.ntile ? (keys + kTileKeys - 1) / kTileKeys : 0;
-  }
+    return (keys + kTileKeys - 1) / kTileKeys;
+  };
+  const int all = blocks(w.ntile - 1);
+  const int j0 = (int)((long long)all * w.split / tg.splits), j1 = (int)((long long)all * (w.split + 1) / tg.splits);
+  for (int t = 0; t < 2; ++t) w.nb[t] = t < w.ntile ? max(0, min(blocks(t), j1) - j0) : 0;
   w.nblk = w.nb[w.ntile - 1];
-  const int all = p.causal ? max(0, min(w.s.nk, w.r0 + off + 1)) : w.s.nk;   // keys that the first row sees
-  w.e0 = min(all / kTileKeys, w.nblk);
+  const int whole = (p.causal ? max(0, min(w.s.nk, w.t0 + off + 1)) : w.s.nk) / kTileKeys;   // blocks the first row sees
+  w.e0 = min(max(whole - j0, 0), w.nblk);
+  w.s.k0 += j0 * kTileKeys;
+  w.s.nk -= j0 * kTileKeys;
   return true;
 }
 
@@ -142,7 +163,7 @@ template <int DP> __device__ __forceinline__ int v_use(int j, int nblk) {
 
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
-    attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const int n_slots, const int negate) {
+    attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const TileGrid tg, const int negate) {
   using Cfg = TileCfg<DP>;
   constexpr int U = Cfg::kUnits, GU = Cfg::kGroup, GN = Cfg::kGroups, NB = Cfg::kSlots * GN;
   constexpr bool kTwo = Cfg::kTiles == 2;
@@ -169,9 +190,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += Cfg::kThreads) attn_seq(p, b, true);
   TileWork w;
-  if (!tile_work<DP>(p, n_slots, w)) return;
+  if (!tile_work<DP>(p, tg, w)) return;
   const Seq s = w.s;
-  const int off = s.nk - s.nq;
+  const int off = s.nk - s.nq;   // the same for a part of the keys, counted from its first
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NB; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -201,10 +222,11 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         tma_prefetch_desc(&maps.q);
         tma_prefetch_desc(&maps.k);
         tma_prefetch_desc(&maps.v);
-        mbar_arrive_expect_tx(q_full, w.ntile * U * kTileUnitBytes);
+        mbar_arrive_expect_tx(q_full, w.ntile * U * tg.tokens * p.G * 128);
         for (int t = 0; t < w.ntile; ++t)
-          for (int u = 0; u < U; ++u)
-            tma_load_3d(q_smem + (t * U + u) * kTileUnitBytes, &maps.q, q_full, u * 64, w.head, s.q0 + w.r0 + t * 128);
+          for (int u = 0; u < U; ++u)   // row token * G + head of the tile
+            tma_load_3d(q_smem + (t * U + u) * kTileUnitBytes, &maps.q, q_full, u * 64, w.kvh * p.G,
+                        s.q0 + w.t0 + t * tg.tokens);
         int edges = 0, uses = 0;
         bool ok = true;
         for (int n = 0; ok && n < 2 * w.nblk; ++n) {
@@ -369,9 +391,12 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     if constexpr (kTwo) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
     const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int row = w.r0 + t * 128 + (warp & 3) * 32 + lane;
-    const int limit = p.causal ? min(s.nk - 1, row + off) : s.nk - 1;                  // last key this row sees
-    const int limit0 = p.causal ? min(s.nk - 1, row - lane + off) : s.nk - 1;          // of the warp's first row
+    const int row = (warp & 3) * 32 + lane;   // of the tile
+    const int tok = w.t0 + t * tg.tokens + row / p.G, head = w.kvh * p.G + row % p.G;
+    const bool real = row < tg.tokens * p.G && tok < s.nq;
+    const int limit = !real ? -1 : p.causal ? min(s.nk - 1, tok + off) : s.nk - 1;   // last key this row sees
+    // of the warp's first row, the least of its real rows
+    const int limit0 = p.causal ? min(s.nk - 1, w.t0 + t * tg.tokens + (row - lane) / p.G + off) : s.nk - 1;
     const float sc = p.scale_log2;
     const float grow = 8.f / sc;
     float m = -INFINITY, l = 0.f;
@@ -473,9 +498,13 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      uint16_t* dst = p.out + (long long)(s.q0 + row) * p.o_st + w.head * p.o_sh;
       const bool odd = *odd_values != 0;
+      const bool direct = tg.splits == 1;
+      const float inv = !direct ? 1.f : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      uint16_t* dst = p.out + (long long)(s.q0 + tok) * p.o_st + head * p.o_sh;
+      // (the unit's number, split, tile and row)
+      float* part = direct ? nullptr
+                           : tg.part + (((long long)blockIdx.x * Cfg::kTiles + t) * 128 + row) * (DP + 2);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
@@ -486,9 +515,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (row < s.nq) {
+        if (real) {
           if (odd) {   // add the values that were taken out, where this row sees them
-            for (int key = w.e0 * kTileKeys; key <= limit; ++key) {
+            for (int key = w.e0 * kTileKeys; key <= min(limit, w.nblk * kTileKeys - 1); ++key) {
               const uint16_t* vr = p.v + (long long)(s.k0 + key) * p.v_st + w.kvh * p.v_sh + c * 32;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -496,17 +525,27 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
                   o[i] = __float_as_uint(__uint_as_float(o[i]) + bits_to_f32(vr[i], BF16 ? kBF16 : kF16));
             }
           }
+          if (direct) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c * 32 + i * 8 < p.D) {
-              uint4 x;
-              x.x = pack2_rn<BF16>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-              x.y = pack2_rn<BF16>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-              x.z = pack2_rn<BF16>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-              x.w = pack2_rn<BF16>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = x;
-            }
+            for (int i = 0; i < 4; ++i)
+              if (c * 32 + i * 8 < p.D) {
+                uint4 x;
+                x.x = pack2_rn<BF16>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+                x.y = pack2_rn<BF16>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+                x.z = pack2_rn<BF16>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+                x.w = pack2_rn<BF16>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+                *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = x;
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              *reinterpret_cast<uint2*>(part + c * 32 + 2 * i) = make_uint2(o[2 * i], o[2 * i + 1]);
+          }
         }
+      }
+      if (!direct && real) {
+        part[DP] = m * sc;
+        part[DP + 1] = l;
       }
     }
   }
@@ -516,6 +555,44 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the keys: one warp per row, 8 rows of a tile to a block. Grid: units x tiles, 16.
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p, const TileGrid tg) {
+  using Cfg = TileCfg<DP>;
+  constexpr int kV = DP / 32;   // columns of a lane
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int unit = blockIdx.x / Cfg::kTiles, t = blockIdx.x - unit * Cfg::kTiles;
+  const int row = blockIdx.y * 8 + warp_id(), lane = lane_id();
+  const int kvh = unit / tg.slots;
+  TileWork w;
+  if (row >= tg.tokens * p.G || !tile_range<DP>(p, tg, tg.slots - 1 - (unit - kvh * tg.slots), w)) return;
+  const int tok = w.t0 + t * tg.tokens + row / p.G;
+  if (tok >= w.s.nq) return;
+  auto part = [&](int z) {
+    return tg.part + ((((long long)unit * tg.splits + z) * Cfg::kTiles + t) * 128 + row) * (DP + 2);
+  };
+  float mx = -INFINITY;
+  for (int z = 0; z < tg.splits; ++z) mx = fmaxf(mx, part(z)[DP]);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f, acc[kV];
+#pragma unroll
+  for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < tg.splits; ++z) {
+    const float* x = part(z);
+    const float f = ex2(x[DP] - ref);
+    l += f * x[DP + 1];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] += f * x[lane * kV + i];
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (lane * kV < p.D) {
+    uint16_t* dst = p.out + (long long)(w.s.q0 + tok) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + lane * kV;
+#pragma unroll
+    for (int i = 0; i < kV; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2_rn<BF16>(acc[i] * inv, acc[i + 1] * inv);
   }
 }
 

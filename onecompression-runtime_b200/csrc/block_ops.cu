@@ -71,7 +71,6 @@ int launch_rope_dt(const oc::RopeParams& p, bool vec, bool inter, int sms, cudaS
 }
 
 // ------------------------------------------------------------------ attention
-constexpr int kTileMinRows = 16;
 int attn_dp(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 template <int DP> int split_ctas(int sms) { return sms * oc::SplitCfg<DP>::kCtasPerSm; }
@@ -81,6 +80,43 @@ int split_ctas(int dp, int sms) {
 size_t split_desc_bytes(int ctas) { return (((size_t)ctas * oc::kSplitDescInts * 4) + 255) / 256 * 256; }
 size_t split_ws_bytes(int dp, int ctas) {
   return split_desc_bytes(ctas) + (size_t)ctas * 2 * oc::kSplitRows * (dp + 2) * 4;
+}
+
+// Which kernel a call takes, and its workspace. The host knows the longest query run (max_q) or, without
+// it, the mean one.
+constexpr int kTileMinRows = 16;
+struct AttnPlan {
+  bool tile;
+  int dp, ctas;      // split kernel: its grid
+  oc::TileGrid tg;
+  size_t ws;
+};
+
+AttnPlan attn_plan(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q, int sms) {
+  AttnPlan pl{};
+  pl.dp = attn_dp(D);
+  const int64_t seqs = std::max(B, 1), G = Hq / Hkv;
+  const int64_t run = max_q > 0 ? std::min(max_q, Tq) : (Tq + seqs - 1) / seqs;
+  // One tile of 16 (token, head) rows streams the keys from memory at the split kernel's rate; more rows are
+  // tensor work.
+  pl.tile = run * G > kTileMinRows && G <= 128 && B > 0 && Tk > 0;
+  if (!pl.tile) {
+    pl.ctas = split_ctas(pl.dp, sms);
+    pl.ws = split_ws_bytes(pl.dp, pl.ctas);
+    return pl;
+  }
+  const int tiles = pl.dp == 256 ? 1 : 2;
+  pl.tg.tokens = 128 / (int)G;
+  const int64_t range = (int64_t)tiles * pl.tg.tokens;
+  pl.tg.slots = (int)(Tq / range) + B;
+  // Ranges that hold tokens, about; with fewer of them than SMs the keys of each are split over several
+  // CTAs, at least two blocks of keys to a part.
+  const int64_t busy = Hkv * std::max(seqs * ((run + range - 1) / range), Tq / range);
+  const int64_t blocks = ((Tk + seqs - 1) / seqs + oc::kTileKeys - 1) / oc::kTileKeys;
+  pl.tg.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / busy, blocks / 2, 32}));
+  if (pl.tg.splits > 1)
+    pl.ws = (size_t)pl.tg.slots * Hkv * pl.tg.splits * tiles * 128 * (pl.dp + 2) * 4;
+  return pl;
 }
 
 template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas, cudaStream_t stream) {
@@ -93,14 +129,15 @@ template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas,
                     "attention (join)", p);
 }
 
-// [rows, heads, D] tensor in boxes of 128 rows x one head x 64 columns. A dimension of one row or head
-// takes any valid stride.
-int attn_tmap(CUtensorMap* map, bool bf16, const void* base, int D, int H, int T, int64_t sh, int64_t st) {
+// [rows, heads, D] tensor in boxes of `rows` rows x `heads` heads x 64 columns. A dimension of one row or
+// head takes any valid stride.
+int attn_tmap(CUtensorMap* map, bool bf16, const void* base, int D, int H, int T, int64_t sh, int64_t st, int heads,
+              int rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(OC_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
   cuuint64_t strides[2] = {(cuuint64_t)(H > 1 ? sh : D) * 2, (cuuint64_t)(T > 1 ? st : D) * 2};
-  cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)rows}, estr[3] = {1, 1, 1};
   const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -109,14 +146,14 @@ int attn_tmap(CUtensorMap* map, bool bf16, const void* base, int D, int H, int T
   return OC_OK;
 }
 
-template <bool BF16, int DP> int launch_tile(oc::AttnParams p, cudaStream_t stream) {
+template <bool BF16, int DP> int launch_tile(oc::AttnParams p, const oc::TileGrid& tg, cudaStream_t stream) {
   using Cfg = oc::TileCfg<DP>;
   oc::TileMaps maps;
-  if (int rc = attn_tmap(&maps.q, BF16, p.q, p.D, p.Hq, p.Tq, p.q_sh, p.q_st)) return rc;
-  if (int rc = attn_tmap(&maps.k, BF16, p.k, p.D, p.Hkv, p.Tk, p.k_sh, p.k_st)) return rc;
-  if (int rc = attn_tmap(&maps.v, BF16, p.v, p.D, p.Hkv, p.Tk, p.v_sh, p.v_st)) return rc;
-  const int slots = p.Tq / Cfg::kRows + p.B;
-  if ((long long)slots * p.Hq > INT_MAX) return fail(OC_ERR_INVALID, "attention: %d tiles x %d heads", slots, p.Hq);
+  if (int rc = attn_tmap(&maps.q, BF16, p.q, p.D, p.Hq, p.Tq, p.q_sh, p.q_st, p.G, tg.tokens)) return rc;
+  if (int rc = attn_tmap(&maps.k, BF16, p.k, p.D, p.Hkv, p.Tk, p.k_sh, p.k_st, 1, oc::kTileKeys)) return rc;
+  if (int rc = attn_tmap(&maps.v, BF16, p.v, p.D, p.Hkv, p.Tk, p.v_sh, p.v_st, 1, oc::kTileKeys)) return rc;
+  const long long units = (long long)tg.slots * p.Hkv;
+  if (units * tg.splits > INT_MAX / 2) return fail(OC_ERR_INVALID, "attention: %lld token ranges", units);
   // the softmax takes its maximum before the scale: a negative scale negates Q in the product, and
   // zero becomes a scale that rounds every finite score to zero but leaves masked ones infinite
   const int negate = p.scale_log2 < 0.f;
@@ -127,8 +164,11 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, cudaStream_t stre
       "attention (tile)");
   if (regs_rc) return fail(regs_rc, "attention (tile): register count of the build");
   if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
-  kern<<<slots * p.Hq, Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, slots, negate);
-  return launch_check("attention (tile)");
+  kern<<<(unsigned)(units * tg.splits), Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, tg, negate);
+  if (int rc = launch_check("attention (tile)")) return rc;
+  if (tg.splits == 1) return OC_OK;
+  return launch_pdl(oc::attn_tile_join_kernel<BF16, DP>, dim3((unsigned)(units * Cfg::kTiles), 16), dim3(256), 0, stream,
+                    "attention (tile join)", p, tg);
 }
 
 // ------------------------------------------------------------------ dense linear
@@ -301,12 +341,11 @@ extern "C" int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_o
   return launch_rope_dt<oc::kF32, 4>(p, vec, interleaved != 0, sms, stream);
 }
 
-extern "C" size_t oc_b200_attention_workspace(int D) {
-  if (D <= 0 || D > 256) return 0;
+extern "C" size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q) {
+  if (Tq <= 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
   int dev = 0;
   if (current_device(&dev)) return 0;
-  const int dp = attn_dp(D);
-  return split_ws_bytes(dp, split_ctas(dp, sm_count(dev)));
+  return attn_plan(Tq, Tk, B, Hq, Hkv, D, max_q, sm_count(dev)).ws;
 }
 
 extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -334,8 +373,10 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
       return fail(OC_ERR_INVALID, "attention: stride %lld (a multiple of 8 elements)", (long long)st);
   int dev = 0;
   if (int rc = current_device(&dev)) return rc;
-  const int dp = attn_dp(D);
-  const int ctas = split_ctas(dp, sm_count(dev));
+  AttnPlan pl = attn_plan(Tq, Tk, B, Hq, Hkv, D, max_q, sm_count(dev));
+  if (pl.ws && (!workspace || workspace_bytes < pl.ws || !aligned(workspace, 16)))
+    return fail(OC_ERR_WORKSPACE, "attention: needs %zu bytes of 16-byte aligned workspace, got %zu", pl.ws,
+                workspace_bytes);
   oc::AttnParams p{};
   p.q = reinterpret_cast<const uint16_t*>(q);
   p.k = reinterpret_cast<const uint16_t*>(Tk > 0 ? k : q);
@@ -351,16 +392,13 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const bool bf16 = dtype == OC_DT_BF16;
-  // Query rows of a sequence, as far as the host knows them.
-  const int64_t run = max_q > 0 ? std::min(max_q, Tq) : ((int64_t)Tq + std::max(B, 1) - 1) / std::max(B, 1);
-  if (run > kTileMinRows && B > 0 && Tk > 0) {
-    if (dp == 64) return bf16 ? launch_tile<true, 64>(p, stream) : launch_tile<false, 64>(p, stream);
-    if (dp == 128) return bf16 ? launch_tile<true, 128>(p, stream) : launch_tile<false, 128>(p, stream);
-    return bf16 ? launch_tile<true, 256>(p, stream) : launch_tile<false, 256>(p, stream);
+  const int dp = pl.dp, ctas = pl.ctas;
+  if (pl.tile) {
+    pl.tg.part = reinterpret_cast<float*>(workspace);
+    if (dp == 64) return bf16 ? launch_tile<true, 64>(p, pl.tg, stream) : launch_tile<false, 64>(p, pl.tg, stream);
+    if (dp == 128) return bf16 ? launch_tile<true, 128>(p, pl.tg, stream) : launch_tile<false, 128>(p, pl.tg, stream);
+    return bf16 ? launch_tile<true, 256>(p, pl.tg, stream) : launch_tile<false, 256>(p, pl.tg, stream);
   }
-  if (!workspace || workspace_bytes < split_ws_bytes(dp, ctas) || !aligned(workspace, 16))
-    return fail(OC_ERR_WORKSPACE, "attention: needs %zu bytes of 16-byte aligned workspace, got %zu",
-                split_ws_bytes(dp, ctas), workspace_bytes);
   p.desc = reinterpret_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + split_desc_bytes(ctas));
   if (dp == 64) return bf16 ? launch_split<true, 64>(p, ctas, stream) : launch_split<false, 64>(p, ctas, stream);

@@ -80,7 +80,7 @@ _SIGNATURES = {
                                             _i),
     "oc_b200_rope": ([_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _i, _p, _i,
                       _i64, _p, _p, ctypes.c_float, _i, _p], _i),
-    "oc_b200_attention_workspace": ([_i], _sz),
+    "oc_b200_attention_workspace": ([_i] * 7, _sz),
     "oc_b200_attention": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _i, _i, _p,
                            _p, _p, _i, _i, ctypes.c_float, _i, _i, _p, _sz, _p], _i),
     "oc_b200_dense_gemm": ([_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i, _p, _i64, _i, _p, _i64, _p], _i),

@@ -1,19 +1,12 @@
 """Attention over packed sequences on B200: prompts, parts of prompts and single tokens."""
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
 
 from .. import _lib
 from ._block_ops import inference_only, on_device, one_device, overlap
-
-
-@functools.lru_cache(maxsize=None)
-def _workspace_bytes(device_index: int, head_dim: int) -> int:
-    with torch.cuda.device(device_index):
-        return _lib.lib().oc_b200_attention_workspace(head_dim)
 
 
 def _rows(t: torch.Tensor, copy: bool = True) -> tuple[torch.Tensor, int, int, int] | None:
@@ -110,9 +103,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_k = None if cu_seqlens_k is None else cu_seqlens_k.contiguous()
     lens = None if kv_lens is None else kv_lens.contiguous()
     with on_device(dev):
-        ws = torch.empty(_workspace_bytes(dev.index, D), dtype=torch.uint8, device=dev)
+        run = 0 if max_seqlen_q is None else max(0, max_seqlen_q)
+        size = _lib.lib().oc_b200_attention_workspace(Tq, Tk, B, Hq, Hkv, D, run)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _lib.call("oc_b200_attention", q_ptr, q_st, q_sh, k_ptr, k_st, k_sh, v_ptr, v_st, v_sh, o_ptr, o_st, o_sh,
                   _lib.DT[dtype], Tq, Tk, Hq, Hkv, D, _lib.ptr(cu_q), _lib.ptr(cu_k), _lib.ptr(lens), B, causal, scale,
-                  0 if max_seqlen_q is None else max(0, max_seqlen_q), out is None, ws.data_ptr(), ws.numel(),
-                  _lib.stream_of(dev))
+                  run, out is None, _lib.ptr(ws), size, _lib.stream_of(dev))
     return target

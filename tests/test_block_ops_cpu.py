@@ -150,7 +150,7 @@ def test_c_entry_points_refuse_before_any_launch():
         assert attn(**kw) == 1, kw
     assert attn(D=60) == 2 and attn(D=264) == 2
     assert attn(Tq=0) == 0 and attn(B=0) == 0
-    assert lib.oc_b200_attention_workspace(0) == 0 and lib.oc_b200_attention_workspace(512) == 0
+    assert lib.oc_b200_attention_workspace(4, 4, 1, 4, 2, 0, 0) == 0 and lib.oc_b200_attention_workspace(4, 4, 1, 4, 3, 64, 0) == 0
 
     def dense(x=p, w=p, dt=1, M=4, N=40, K=64, ldx=64, act=0, bdt=0, ldc=40, c=p, res=None, ldr=0, bias=None):
         return lib.oc_b200_dense_gemm(x, ldx, w, 64, dt, M, N, K, bias, bdt, res, ldr, act, c, ldc, None)
