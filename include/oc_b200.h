@@ -317,8 +317,7 @@ int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t
  * 16-byte aligned, D a multiple of 8 up to 256. Sequence b: query rows cu_q[b] .. cu_q[b+1], key rows
  * from cu_k[b], kv_lens[b] of them (NULL: up to cu_k[b+1]); cu_q = cu_k = NULL: one sequence of all
  * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros.
- * Query rows outside every sequence stay as they were, or become zeros with zero_tail (rows behind
- * cu_q[B]). The tables are read on the device; values outside the tensors are clamped and set the
+ * Query rows outside every sequence stay as they were, or become zeros with zero_unowned. The tables are read on the device; values outside the tensors are clamped and set the
  * device error word. max_q (0: unknown) is a hint of the longest query run; it only picks a kernel.
  * workspace: oc_b200_attention_workspace bytes for the same sizes on the current device (may be 0), any
  * contents, 16-byte aligned, not shared by calls that may run at once. out must not overlap the inputs. */
@@ -326,7 +325,7 @@ size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D
 int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                       const void* v, int64_t v_st, int64_t v_sh, void* out, int64_t o_st, int64_t o_sh, int dtype,
                       int Tq, int Tk, int Hq, int Hkv, int D, const int32_t* cu_q, const int32_t* cu_k,
-                      const int32_t* kv_lens, int B, int causal, float scale, int max_q, int zero_tail,
+                      const int32_t* kv_lens, int B, int causal, float scale, int max_q, int zero_unowned,
                       void* workspace, size_t workspace_bytes, oc_stream_t stream);
 /* Dense linear: C[M, N] = act(X[M, K] W[N, K]^T + bias) + residual, f16 or bf16 with fp32
  * accumulation and epilogue, one rounding. K a multiple of 8, X and W rows 16-byte aligned; bias

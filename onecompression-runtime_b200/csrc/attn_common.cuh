@@ -23,7 +23,7 @@ struct AttnParams {
   const int* kv_lens;   // [B] or null
   int B;
   int causal;
-  int zero_tail;        // also write zeros to the query rows that no sequence owns
+  int zero_unowned;     // also write zeros to the query rows that no sequence owns
   float scale_log2;     // softmax scale * log2(e)
   float* part;          // split kernel: partial results
   int* desc;            // split kernel: one descriptor per CTA
@@ -52,17 +52,19 @@ __device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report 
   return s;
 }
 
-// The first query row behind the last sequence.
-__device__ __forceinline__ int attn_tail(const AttnParams& p) {
-  return p.cu_q ? min(max(p.cu_q[p.B], 0), p.Tq) : p.Tq;
-}
-
-// One CTA's share of the rows that no sequence owns: zeros (D is a multiple of 8, rows 16-byte aligned).
-__device__ __forceinline__ void attn_zero_tail(const AttnParams& p, int cta, int n_ctas) {
+// One CTA's share of the rows that no sequence owns, in front of the first one and behind the last: zeros
+// (D is a multiple of 8, rows 16-byte aligned).
+__device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, int n_ctas) {
+  if (!p.cu_q) return;
   const int vecs = p.D / 8;
-  for (long long t = (long long)attn_tail(p) + cta; t < p.Tq; t += n_ctas)
+  const int head = p.B > 0 ? min(max(p.cu_q[0], 0), p.Tq) : 0;
+  const int tail = min(max(p.cu_q[p.B], head), p.Tq);
+  const long long rows = (long long)head + (p.Tq - tail);
+  for (long long r = cta; r < rows; r += n_ctas) {
+    const long long t = r < head ? r : tail + (r - head);
     for (int i = threadIdx.x; i < p.Hq * vecs; i += blockDim.x)
       *reinterpret_cast<uint4*>(p.out + t * p.o_st + (i / vecs) * p.o_sh + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -90,39 +92,10 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-// 2^x of a pair on the FMA pipe, beside the 16 a cycle and SM that ex2.approx gives: x = n + f with n the
-// nearest integer (the magic sum 1.5 2^23 + x keeps n in its low bits), 2^f on [-1/2, 1/2] by the
-// polynomial of degree 4 with the least largest relative error (Remez exchange; 2.6e-6), times 2^n built
-// in the exponent field. NaN stays NaN; x is clamped to -126 from below, x above 127 does not occur.
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
-  float a, b;
-  f2_unpack(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-  x = f2_pack(a, b);
-  const uint64_t magic = f2_pack(12582912.f, 12582912.f), neg = f2_pack(-12582912.f, -12582912.f);
-  const uint64_t n = f2_add(x, magic);
-  const uint64_t f = f2_fma(f2_add(n, neg), f2_pack(-1.f, -1.f), x);
-  uint64_t r = f2_pack(0.009570102207362652f, 0.009570102207362652f);
-  r = f2_fma(r, f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
-  r = f2_fma(r, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-  r = f2_fma(r, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-  r = f2_fma(r, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-  f2_unpack(n, a, b);
-  const float sa = __int_as_float((__float_as_int(a) << 23) + 0x3f800000);
-  const float sb = __int_as_float((__float_as_int(b) << 23) + 0x3f800000);
-  return f2_mul(r, f2_pack(sa, sb));
 }
 
 // Is one of the two 16-bit values of a register infinite or NaN?

@@ -26,8 +26,6 @@
 // (common.cuh).
 #pragma once
 
-#include <type_traits>
-
 #include "attn_common.cuh"
 
 namespace oc {
@@ -35,18 +33,6 @@ namespace oc {
 constexpr int kTileKeys = 128;
 constexpr int kTileUnitBytes = 128 * 128;   // [128 rows x 64 columns] of 16-bit values
 constexpr int kTileMaxEdges = 3;
-#ifndef OC_ATTN_POLY
-#define OC_ATTN_POLY 0
-#endif
-#ifndef OC_ATTN_PART
-#define OC_ATTN_PART 3
-#endif
-#ifndef OC_ATTN_IN_ORDER
-#define OC_ATTN_IN_ORDER 0
-#endif
-constexpr int kTilePart = OC_ATTN_PART;     // of 4 chunks of 32 keys, those whose product starts ahead of the rest
-constexpr int kTilePoly = OC_ATTN_POLY;     // of 16 pairs of exponentials, those on the FMA pipe
-
 template <int DP> struct TileCfg {
   static constexpr int kTiles = DP == 256 ? 1 : 2;          // row tiles of a CTA
   static constexpr int kRows = kTiles * 128;
@@ -175,7 +161,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   uint64_t* empty = full + NB;
   uint64_t* q_full = empty + NB;
   uint64_t* s_full = q_full + 1;            // [2] by tile, or by block parity where there is one tile
-  uint64_t* p_part = s_full + 2;            // [2] the first 32 * kTilePart keys' weights are there
+  uint64_t* p_part = s_full + 2;            // [2] the first 36 keys' weights are there
   uint64_t* p_full = p_part + 2;            // [2] all are
   uint64_t* pv_done = p_full + 2;           // [2] by tile
   uint64_t* edge_full = pv_done + 2;        // [3] V blocks from e0 on: loaded
@@ -186,7 +172,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   volatile int* odd_values = abort_flag + 1;   // an infinity or NaN was taken out of a V block
   const int warp = warp_uniform(warp_id()), lane = lane_id();
 
-  if (p.zero_tail) attn_zero_tail(p, blockIdx.x, gridDim.x);
+  if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x);
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += Cfg::kThreads) attn_seq(p, b, true);
   TileWork w;
@@ -314,7 +300,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int k = h ? 2 * kTilePart : 0; k < (h ? 8 : 2 * kTilePart); ++k)
+            for (int k = h ? 6 : 0; k < (h ? 8 : 6); ++k)
               tc_mma_ts(tm + Cfg::o_col(t), tm + Cfg::p_col(b) + k * 8, vd + k * (2048 / 16), idesc_pv,
                         (j | k) != 0 ? 1u : 0u);
             if (h) {
@@ -339,10 +325,10 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         if (ok && last_tile && nblk > 0) ok = qk(1, 0, nb0 == 0);
         for (int j = 0; ok && j < nblk; ++j) {
           if (j < nb0) ok = pv(0, j, true);
-          if (ok && j + 1 < nb0) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(0, j)) && qk(0, j + 1, true);
+          if (ok && j + 1 < nb0) ok = (DP == 64 || pv_over(0, j)) && qk(0, j + 1, true);
           if (!last_tile) continue;
           if (ok) ok = pv(1, j, j >= nb0);
-          if (ok && j + 1 < nblk) ok = (OC_ATTN_IN_ORDER || DP == 64 || pv_over(1, j)) && qk(1, j + 1, j + 1 >= nb0);
+          if (ok && j + 1 < nblk) ok = (DP == 64 || pv_over(1, j)) && qk(1, j + 1, j + 1 >= nb0);
         }
       } else {
         if (nblk > 0) ok = ok && qk(0, 0, true);
@@ -453,40 +439,29 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       }
       const float bias = m == -INFINITY ? 0.f : -m * sc;
       const uint64_t sc2 = f2_pack(sc, sc), bias2 = f2_pack(bias, bias);
+      // (a polynomial on the FMA pipe for 2 of every 16 pairs, to relieve the exponential unit, lengthened the
+      // chain: 3.52 ms against 3.44 at 16384 tokens, 32 heads of 128)
       uint64_t sum = 0;   // (0.f, 0.f)
-      // Of every 16 pairs kTilePoly go through the polynomial, so that neither the exponential unit nor
-      // the FMA pipe is waited for; blocks with masked scores take ex2, which gives them exact zeros.
-      auto weights = [&](auto poly) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t x =
-                f2_fma(f2_pack(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, bias2);
-            float p0, p1;
-            uint64_t w2;
-            if (poly && i * kTilePoly % 16 < kTilePoly) {
-              w2 = ex2_poly2(x);
-              f2_unpack(w2, p0, p1);
-            } else {
-              f2_unpack(x, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-              w2 = f2_pack(p0, p1);
-            }
-            sum = f2_add(sum, w2);
-            pk[i] = pack2_rn<BF16>(p0, p1);
-          }
-          tmem_st_32x32b_x16(tmem + lanes + Cfg::p_col(b) + c * 16, pk);
-          if (c == kTilePart - 1 || c == 3) {
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(c == 3 ? &p_full[b] : &p_part[b]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t x = f2_fma(f2_pack(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, bias2);
+          float p0, p1;
+          f2_unpack(x, p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum = f2_add(sum, f2_pack(p0, p1));
+          pk[i] = pack2_rn<BF16>(p0, p1);
         }
-      };
-      if (edge) weights(std::false_type{}); else weights(std::true_type{});
+        tmem_st_32x32b_x16(tmem + lanes + Cfg::p_col(b) + c * 16, pk);
+        if (c >= 2) {   // 96 keys' weights: the product starts; then the rest
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(c == 3 ? &p_full[b] : &p_part[b]);
+        }
+      }
       float s0, s1;
       f2_unpack(sum, s0, s1);
       l += s0 + s1;

@@ -352,7 +352,7 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
                                  const void* v, int64_t v_st, int64_t v_sh, void* out, int64_t o_st, int64_t o_sh,
                                  int dtype, int Tq, int Tk, int Hq, int Hkv, int D, const int32_t* cu_q,
                                  const int32_t* cu_k, const int32_t* kv_lens, int B, int causal, float scale,
-                                 int max_q, int zero_tail, void* workspace, size_t workspace_bytes,
+                                 int max_q, int zero_unowned, void* workspace, size_t workspace_bytes,
                                  oc_stream_t stream_) {
   if (!dt16(dtype)) return fail(OC_ERR_INVALID, "attention: dtype %d (f16 or bf16)", dtype);
   if (Tq < 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
@@ -361,8 +361,8 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
     return fail(OC_ERR_UNSUPPORTED, "attention: head size %d (a multiple of 8 up to 256)", D);
   if ((cu_q == nullptr) != (cu_k == nullptr)) return fail(OC_ERR_INVALID, "attention: cu_q and cu_k come together");
   if (!cu_q && B != 1) return fail(OC_ERR_INVALID, "attention: B=%d without sequence tables", B);
-  if (!std::isfinite(scale)) return fail(OC_ERR_INVALID, "attention: scale %g", (double)scale);
-  if (Tq == 0 || (B == 0 && !zero_tail)) return OC_OK;
+  if (!std::isfinite(scale * 1.4426950408889634f)) return fail(OC_ERR_INVALID, "attention: scale %g", (double)scale);
+  if (Tq == 0 || (B == 0 && !zero_unowned)) return OC_OK;
   if (!q || !out || (Tk > 0 && (!k || !v))) return fail(OC_ERR_INVALID, "attention: NULL pointer");
   const void* ptrs[4] = {q, Tk > 0 ? k : q, Tk > 0 ? v : q, out};
   const int64_t strides[8] = {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh};
@@ -388,7 +388,7 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   p.cu_q = cu_q; p.cu_k = cu_k; p.kv_lens = kv_lens;
   p.B = B;
   p.causal = causal != 0;
-  p.zero_tail = zero_tail != 0;
+  p.zero_unowned = zero_unowned != 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const bool bf16 = dtype == OC_DT_BF16;

@@ -52,7 +52,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     result, not even infinities or NaN. ``scale`` defaults to ``D ** -0.5``. ``max_seqlen_q``: the longest
     query run if the host knows it; it only helps to pick the kernel (results are right whatever it says).
     ``out``: [Tq, Hq, D] to write into, sharing no memory with the inputs; rows that no sequence owns stay as
-    they were (a new output holds zeros behind the last sequence).
+    they were (a new output holds zeros there).
     """
     what = "packed_attention"
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
@@ -91,6 +91,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if rows_out is None:
             raise ValueError(f"{what}: out needs a unit last stride and 16-byte aligned rows")
         target, o_ptr, o_st, o_sh = rows_out
+        (s0, n0), (s1, n1) = sorted(((o_st, Tq), (o_sh, Hq)))
+        if (n0 > 1 and s0 < D) or (n1 > 1 and s1 < (s0 * (n0 - 1) + D if n0 > 1 else D)):
+            raise ValueError(f"{what}: out rows overlap (strides {out.stride()})")
     else:
         target = torch.empty((Tq, Hq, D), dtype=dtype, device=dev)
         o_ptr, o_st, o_sh = target.data_ptr(), Hq * D, D

@@ -209,6 +209,77 @@ def test_attention_out_and_rows_of_no_sequence(cuda_device):
         assert bool((got[n:] == 7).all()) and bool((buf[..., :64] == 7).all()) and bool((fresh[n:] == 0).all())
 
 
+def test_attention_rows_in_front_of_the_first_sequence(cuda_device):
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    for first, lq in ((2, [3, 2]), (70, [150, 77])):
+        T = first + sum(lq) + 5
+        q, k, v = randn(dev, T, 4, 64, seed=1), randn(dev, T, 4, 64, seed=2), randn(dev, T, 4, 64, seed=3)
+        c = cu(dev, [first, *lq])[1:].contiguous()
+        with torch.no_grad():
+            junk = torch.full((T, 4, 64), math.nan, dtype=BF, device=dev)   # what a new output may hold
+            del junk
+            o = packed_attention(q, k, v, c, c)
+        s0 = first + lq[0]
+        want, tol = ref.attention(q, k, v, [(first, lq[0], first, lq[0]), (s0, lq[1], s0, lq[1])], True, 0.125)
+        ref.check(o, want, tol, "rows in front")
+        assert bool((o[:first] == 0).all()) and bool((o[-5:] == 0).all())
+
+
+@pytest.mark.parametrize("case", [([20], [3000], 8, 1, 128), ([33, 5], [4001, 90], 6, 2, 64), ([64], [2500], 3, 1, 256),
+                                  ([9, 9, 1, 40], [700, 9, 1, 5000], 10, 2, 128), ([130], [130], 12, 4, 64)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_keys_split_over_ctas(cuda_device, case, dtype):
+    """Few tiles and many keys: parts of the keys on several CTAs, parts that some rows do not see at all, a
+    group that does not divide a tile."""
+    lq, lk, Hq, Hkv, D = case
+    for causal in (True, False):
+        run_attention(cuda_device, lq, lk, Hq, Hkv, D, dtype, causal, seed=5, max_q=max(lq))
+
+
+@pytest.mark.parametrize("G", [3, 7, 20, 64, 100, 128, 130, 200])
+def test_attention_wide_groups(cuda_device, G):
+    run_attention(cuda_device, [3, 40, 1], [50, 300, 1], G, 1, 64, seed=G)
+    run_attention(cuda_device, [1, 1], [700, 3], 2 * G, 2, 64, HF, seed=G, max_q=1)
+
+
+def test_attention_offsets_beyond_32_bits(cuda_device):
+    """Key rows whose element offset passes 2^31, for single tokens and for a prompt; the same for queries."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    st, T, n = 65536, 40000, 300
+    buf = torch.empty(st * T, dtype=BF, device=dev)
+    k, v = buf.as_strided((T, 1, 64), (st, 64, 1)), buf.as_strided((T, 1, 64), (st, 64, 1), 128)
+    k[-n:] = randn(dev, n, 1, 64, seed=1)
+    v[-n:] = randn(dev, n, 1, 64, seed=2)
+    ck = torch.tensor([T - n, T], dtype=torch.int32, device=dev)
+    for nq in (1, 200):
+        q = randn(dev, nq, 4, 64, seed=3)
+        cq = cu(dev, [nq])
+        with torch.no_grad():
+            o = packed_attention(q, k, v, cq, ck)
+            ref.check(o, *ref.attention(q, k[-n:], v[-n:], [(0, nq, 0, n)], True, 0.125), "far keys")
+            wide = k[-nq:]                                   # as queries: rows far apart, far into the buffer
+            far = packed_attention(k, k[-n:], v[-n:], torch.tensor([T - nq, T], dtype=torch.int32, device=dev),
+                                   cu(dev, [n]))[-nq:]
+            ref.check(far, *ref.attention(wide.contiguous(), k[-n:], v[-n:], [(0, nq, 0, n)], True, 0.125), "far queries")
+    assert error_word(dev) == 0
+
+
+def test_attention_refuses_bad_outputs(cuda_device):
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    q = randn(dev, 6, 4, 64)
+    base = torch.empty((6, 4, 65), dtype=BF, device=dev)
+    with torch.no_grad():
+        for out in (q, base[..., 1:], base[..., :64], torch.empty((1, 4, 64), dtype=BF, device=dev).expand(6, 4, 64),
+                    torch.empty(1000, dtype=BF, device=dev).as_strided((6, 4, 64), (64, 8, 1)), q.new_empty(6, 4, 32)):
+            with pytest.raises(ValueError):
+                packed_attention(q, q, q, out=out)
+        with pytest.raises(ValueError, match="tensors on"):
+            packed_attention(q, q.cpu(), q)
+
+
 def test_attention_empty_calls(cuda_device):
     from onecomp_runtime.layers import packed_attention
     dev = cuda_device
