@@ -574,10 +574,12 @@ def bench_cfg4(args, job: Job, peaks: dict, with_cpu: bool) -> dict:
 class DiTStack:
     """8 FLUX-style blocks of FusedInt4Linear layers (random packed weights), one per GPU."""
 
-    def __init__(self, job: Job, blocks: int, timer: LaunchTimer):
-        from onecomp_runtime.layers import FusedInt4Linear
+    def __init__(self, job: Job, blocks: int, timer: LaunchTimer, attention: bool = False):
+        from onecomp_runtime.layers import FusedInt4Linear, RotaryEmbedding
         from onecomp_runtime.testing import CFG1, CFG1_LAYERS, gptq_layer
         gs = CFG1["gs"]
+        # --attention: rotary positions (three axes over a head of 128) and full attention on the qkv output
+        self.rope = RotaryEmbedding(128, axes=[16, 56, 56], layout="interleaved", device=job.dev) if attention else None
         self.blocks = []
         for b in range(blocks):
             blk = {}
@@ -589,14 +591,28 @@ class DiTStack:
         self.hidden = CFG1["hidden"]
 
     def forward(self, h: torch.Tensor) -> torch.Tensor:
-        """q = qkv(h)[:, :H]; h = rms(h + proj(q)); h = rms(h + fc2(gelu(fc1(h)))), adds/GELU in epilogues."""
+        """a = qkv(h)[:, :H], or attention over qkv(h) with --attention; h = rms(h + proj(a));
+        h = rms(h + fc2(gelu(fc1(h)))), adds/GELU in epilogues."""
         H = self.hidden
         for blk in self.blocks:
             qkv = blk["qkv"](h)
-            h = rms_norm(blk["proj"].forward_fused(qkv[:, :H], residual=h))
+            a = qkv[:, :H] if self.rope is None else self.attend(qkv)
+            h = rms_norm(blk["proj"].forward_fused(a, residual=h))
             f = blk["fc1"].forward_fused(h, activation="gelu_tanh")
             h = rms_norm(blk["fc2"].forward_fused(f, residual=h))
         return h
+
+
+    def attend(self, qkv: torch.Tensor) -> torch.Tensor:
+        """Rotary positions in place on the q and k columns, then attention of all tokens on all tokens."""
+        from onecomp_runtime.layers import packed_attention
+        T, H = qkv.shape[0], self.hidden
+        q, k, v = (qkv[:, i * H:(i + 1) * H].unflatten(1, (H // 128, 128)) for i in range(3))
+        if getattr(self, "positions", None) is None or self.positions.shape[0] != T:
+            t = torch.arange(T, device=qkv.device)
+            self.positions = torch.stack([torch.zeros_like(t), t // 64, t % 64], 1)
+        self.rope(q, k, self.positions, inplace=True)
+        return packed_attention(q, k, v, causal=False).flatten(1)
 
 
 def bench_cfg1(args, job: Job, peaks: dict, full_line: bool) -> dict:
@@ -606,7 +622,7 @@ def bench_cfg1(args, job: Job, peaks: dict, full_line: bool) -> dict:
         from onecomp_runtime import _lib
         _lib.set_option(_lib.OPT_TC_TILE, args.tc_tile)
     timer = LaunchTimer()
-    stack = DiTStack(job, blocks, timer)
+    stack = DiTStack(job, blocks, timer, args.attention)
     x = torch.randn(M, CFG1["hidden"], generator=torch.Generator(device=job.dev).manual_seed(1234 + job.rank),
                     device=job.dev).to(torch.bfloat16)
     steps = args.steps if full_line else max(args.steps, 10)
@@ -627,6 +643,8 @@ def bench_cfg1(args, job: Job, peaks: dict, full_line: bool) -> dict:
                                   "fc1 3072->9216, fc2 9216->3072), GPTQ v1 gs32, M=4608 tokens per GPU",
                       "global_batch_tokens": M * job.world, "tokens_per_gpu": M, "blocks": blocks,
                       "parallelism": f"replicas x{job.world} (weak scaling, no collective)",
+                      "attention": ("rotary positions and full attention, 24 heads of 128" if args.attention
+                                    else "none: the q slice stands in"),
                       "l2_flush": "none needed: weights 437 MB packed per stack > 126 MB L2"},
            "gpu_launches": launches,
            "roofline": roofline_tensor(gemm_ms, gemm_flops, peaks, clk, TC_TRAFFIC_CFG1 if not args.blocks else None,
@@ -874,6 +892,8 @@ def main():
                     help="cfg2: OC_OPT_GEMV_PREP (-1 = library default: the integer GEMV prepares its activations "
                          "in each CTA at M <= 2)")
     ap.add_argument("--blocks", type=int, default=0, help="override the number of DiT blocks (profiling only)")
+    ap.add_argument("--attention", action="store_true",
+                    help="cfg1 only: run rotary positions and attention where the q slice stands in by default")
     ap.add_argument("--moe-experts", type=int, default=0, help="cfg3: override the expert count (profiling only)")
     ap.add_argument("--moe-tokens", type=int, default=0, help="cfg3: override tokens per GPU (profiling only)")
     ap.add_argument("--moe-no-fuse", action="store_true",
