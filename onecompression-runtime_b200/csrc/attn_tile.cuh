@@ -91,7 +91,8 @@ struct TileGrid {
   int tokens;    // of a tile: 128 / G
   int slots;     // CTAs' token ranges over all sequences, ragged ends included
   int splits;    // CTAs that share the keys of a range
-  float* part;   // splits > 1: [slot, key head][split][tile][128 rows] O [DP], then m, l
+  float* part;   // splits > 1: [key head, slot][split][tile], each O [DP][128 rows], m [128], l [128]: a warp's rows
+                 // lie side by side (row by row, 8-byte stores 520 B apart doubled the time of a split prompt)
 };
 
 // What a CTA works on; every role derives the same numbers. With a split, the keys are those of its part:
@@ -477,9 +478,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       const bool direct = tg.splits == 1;
       const float inv = !direct ? 1.f : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       uint16_t* dst = p.out + (long long)(s.q0 + tok) * p.o_st + head * p.o_sh;
-      // (the unit's number, split, tile and row)
-      float* part = direct ? nullptr
-                           : tg.part + (((long long)blockIdx.x * Cfg::kTiles + t) * 128 + row) * (DP + 2);
+      float* part = direct ? nullptr : tg.part + ((long long)blockIdx.x * Cfg::kTiles + t) * (128 * (DP + 2)) + row;
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
@@ -513,14 +512,13 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
               }
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              *reinterpret_cast<uint2*>(part + c * 32 + 2 * i) = make_uint2(o[2 * i], o[2 * i + 1]);
+            for (int i = 0; i < 32; ++i) part[(c * 32 + i) * 128] = __uint_as_float(o[i]);
           }
         }
       }
       if (!direct && real) {
-        part[DP] = m * sc;
-        part[DP + 1] = l;
+        part[DP * 128] = m * sc;
+        part[(DP + 1) * 128] = l;
       }
     }
   }
@@ -533,24 +531,26 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   }
 }
 
-// Joins the parts of the keys: one warp per row, 8 rows of a tile to a block. Grid: units x tiles, 16.
+// Joins the parts of the keys, in order: a lane per row, a warp per 8 columns. Grid: units x tiles, 4 groups of 32
+// rows, DP / 64 groups of columns.
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p, const TileGrid tg) {
   using Cfg = TileCfg<DP>;
-  constexpr int kV = DP / 32;   // columns of a lane
+  constexpr int kV = 8;   // columns of a thread
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = blockIdx.x / Cfg::kTiles, t = blockIdx.x - unit * Cfg::kTiles;
-  const int row = blockIdx.y * 8 + warp_id(), lane = lane_id();
+  const int row = blockIdx.y * 32 + lane_id(), col = blockIdx.z * 64 + warp_id() * kV;
   const int kvh = unit / tg.slots;
   TileWork w;
   if (row >= tg.tokens * p.G || !tile_range<DP>(p, tg, tg.slots - 1 - (unit - kvh * tg.slots), w)) return;
   const int tok = w.t0 + t * tg.tokens + row / p.G;
-  if (tok >= w.s.nq) return;
+  if (tok >= w.s.nq || col >= p.D) return;
   auto part = [&](int z) {
-    return tg.part + ((((long long)unit * tg.splits + z) * Cfg::kTiles + t) * 128 + row) * (DP + 2);
+    return tg.part + (((long long)unit * tg.splits + z) * Cfg::kTiles + t) * (128 * (DP + 2)) + row;
   };
   float mx = -INFINITY;
-  for (int z = 0; z < tg.splits; ++z) mx = fmaxf(mx, part(z)[DP]);
+#pragma unroll 4
+  for (int z = 0; z < tg.splits; ++z) mx = fmaxf(mx, part(z)[DP * 128]);
   const float ref = mx == -INFINITY ? 0.f : mx;
   float l = 0.f, acc[kV];
 #pragma unroll
@@ -558,17 +558,16 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p,
 #pragma unroll 4
   for (int z = 0; z < tg.splits; ++z) {
     const float* x = part(z);
-    const float f = ex2(x[DP] - ref);
-    l += f * x[DP + 1];
+    const float f = ex2(x[DP * 128] - ref);
+    l += f * x[(DP + 1) * 128];
 #pragma unroll
-    for (int i = 0; i < kV; ++i) acc[i] += f * x[lane * kV + i];
+    for (int i = 0; i < kV; ++i) acc[i] += f * x[(col + i) * 128];
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (lane * kV < p.D) {
-    uint16_t* dst = p.out + (long long)(w.s.q0 + tok) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + lane * kV;
-#pragma unroll
-    for (int i = 0; i < kV; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2_rn<BF16>(acc[i] * inv, acc[i + 1] * inv);
-  }
+  uint16_t* dst = p.out + (long long)(w.s.q0 + tok) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + col;
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(pack2_rn<BF16>(acc[0] * inv, acc[1] * inv), pack2_rn<BF16>(acc[2] * inv, acc[3] * inv),
+                 pack2_rn<BF16>(acc[4] * inv, acc[5] * inv), pack2_rn<BF16>(acc[6] * inv, acc[7] * inv));
 }
 
 }  // namespace oc

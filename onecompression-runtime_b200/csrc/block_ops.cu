@@ -1,6 +1,7 @@
 // C ABI of the operators between and beside the packed linears of a transformer block: rotary
 // positions, attention over packed sequences, the dense 16-bit linear.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -26,10 +27,18 @@ int block_ops_device_error(unsigned* value, cudaStream_t stream) {
 
 namespace {
 
-// Raises a kernel's dynamic shared memory limit: an attribute per device, so set on every launch.
-template <typename K> int set_smem(K kern, int bytes) {
-  return cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                    "shared memory limit");
+// Raises a kernel's dynamic shared memory limit, an attribute per device: set once on each, remembered in
+// the launcher's own word.
+template <typename K> int set_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit & done.load(std::memory_order_relaxed)) return OC_OK;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                          "shared memory limit"))
+    return rc;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return OC_OK;
 }
 
 // A kernel that moves registers between its warpgroups (setmaxnreg) waits for ever if the launch gives it
@@ -121,7 +130,8 @@ AttnPlan attn_plan(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q, int
 
 template <bool BF16, int DP> int launch_split(const oc::AttnParams& p, int ctas, cudaStream_t stream) {
   auto kern = oc::attn_split_kernel<BF16, DP>;
-  if (int rc = set_smem(kern, oc::SplitCfg<DP>::kRingBytes)) return rc;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = set_smem(kern, oc::SplitCfg<DP>::kRingBytes, smem_set)) return rc;
   kern<<<ctas, oc::SplitCfg<DP>::kThreads, oc::SplitCfg<DP>::kRingBytes, stream>>>(p);
   if (int rc = launch_check("attention (split)")) return rc;
   return launch_pdl(oc::attn_join_kernel<BF16, DP>, dim3((unsigned)ctas, oc::kSplitRows / 4), dim3(oc::kJoinThreads), 0,
@@ -163,11 +173,12 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, const oc::TileGri
       kern, Cfg::kThreads, Cfg::kTiles == 2 ? Cfg::kSoftmaxThreads * Cfg::kSoftmaxRegs + 128 * Cfg::kAuxRegs : 0,
       "attention (tile)");
   if (regs_rc) return fail(regs_rc, "attention (tile): register count of the build");
-  if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = set_smem(kern, Cfg::kSmem, smem_set)) return rc;
   kern<<<(unsigned)(units * tg.splits), Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, tg, negate);
   if (int rc = launch_check("attention (tile)")) return rc;
   if (tg.splits == 1) return OC_OK;
-  return launch_pdl(oc::attn_tile_join_kernel<BF16, DP>, dim3((unsigned)(units * Cfg::kTiles), 16), dim3(256), 0, stream,
+  return launch_pdl(oc::attn_tile_join_kernel<BF16, DP>, dim3((unsigned)(units * Cfg::kTiles), 4, DP / 64), dim3(256), 0, stream,
                     "attention (tile join)", p, tg);
 }
 
@@ -188,7 +199,8 @@ int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, o
   while (S < 8 && tiles * S * 2 <= slots && kb >= S * 2 * 2) S *= 2;
   if (tiles * S > INT_MAX) return fail(OC_ERR_INVALID, "dense_gemm: %lld tiles", tiles);
   auto kern = oc::dense_split_kernel<BF16, BN>;
-  if (int rc = set_smem(kern, Cfg::kSmem)) return rc;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = set_smem(kern, Cfg::kSmem, smem_set)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * S));
   cfg.blockDim = dim3(oc::kDsThreads);
@@ -251,7 +263,8 @@ int launch_dense_tile(const void* x, int64_t ldx, const void* w, int64_t ldw, co
         return rc;
   }
   auto kern = oc::dense_tile_kernel<BF16, ACT, RES>;
-  if (int rc = set_smem(kern, oc::kDtSmem)) return rc;
+  static std::atomic<uint64_t> smem_set{0};
+  if (int rc = set_smem(kern, oc::kDtSmem, smem_set)) return rc;
   const int pairs = (int)std::min<long long>(tiles, max_pairs);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
