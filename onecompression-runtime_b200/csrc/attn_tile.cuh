@@ -7,7 +7,7 @@
 //   * A softmax warpgroup per tile, one thread per row: it reads S from TMEM (no shuffles), writes the
 //     16-bit weights P back to TMEM as the A operand of the second product, and keeps maximum and sum
 //     in registers. Each tile's products are issued by a thread of their own: while one tile is in its
-//     softmax the tensor pipe runs the other's, and the second product starts on the first 64 keys'
+//     softmax the tensor pipe runs the other's, and the second product starts on the first 96 keys'
 //     weights while the softmax works on the rest.
 //   * The reference that the exponents are taken against follows the running maximum only when
 //     it grows by more than 2^8: weights up to 256 are as exact in 16 bits as weights up to 1, and
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   uint64_t* empty = full + NB;
   uint64_t* q_full = empty + NB;
   uint64_t* s_full = q_full + 1;            // [2] by tile, or by block parity where there is one tile
-  uint64_t* p_part = s_full + 2;            // [2] the first 36 keys' weights are there
+  uint64_t* p_part = s_full + 2;            // [2] the first 96 keys' weights are there
   uint64_t* p_full = p_part + 2;            // [2] all are
   uint64_t* pv_done = p_full + 2;           // [2] by tile
   uint64_t* edge_full = pv_done + 2;        // [3] V blocks from e0 on: loaded

@@ -76,8 +76,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                        ("kv_lens", kv_lens, B)):
         if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or n < 1):
             raise ValueError(f"{what}: {name} must be int32 [{max(n, 1)}], got {t.dtype} {tuple(t.shape)}")
-    if scale is None:
-        scale = D ** -0.5
+    scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: scale {scale}")
     if out is not None and (out.shape != q.shape or out.dtype != dtype):
@@ -106,7 +105,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_k = None if cu_seqlens_k is None else cu_seqlens_k.contiguous()
     lens = None if kv_lens is None else kv_lens.contiguous()
     with on_device(dev):
-        run = 0 if max_seqlen_q is None else max(0, max_seqlen_q)
+        run = 0 if max_seqlen_q is None else min(max(0, int(max_seqlen_q)), Tq)
         size = _lib.lib().oc_b200_attention_workspace(Tq, Tk, B, Hq, Hkv, D, run)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _lib.call("oc_b200_attention", q_ptr, q_st, q_sh, k_ptr, k_st, k_sh, v_ptr, v_st, v_sh, o_ptr, o_st, o_sh,

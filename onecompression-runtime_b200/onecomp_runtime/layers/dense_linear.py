@@ -99,6 +99,7 @@ class EagerLinear(torch.nn.Linear):
 
     def forward_fused(self, x: torch.Tensor, residual: torch.Tensor | None = None,
                       activation: str | None = None) -> torch.Tensor:
-        """``act(x @ W.T + bias) + residual`` in one kernel (:func:`linear_fused`), one rounding."""
+        """``act(x @ W.T + bias) + residual`` in one kernel (:func:`linear_fused`, whose dtypes and multiple of 8
+        input features it needs), one rounding."""
         bias = None if self.bias is None else self.bias.detach()
         return linear_fused(x, self.weight.detach(), bias, activation=activation, residual=residual)

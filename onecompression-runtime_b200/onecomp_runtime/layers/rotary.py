@@ -188,6 +188,8 @@ class RotaryEmbedding(torch.nn.Module):
         T = q_shape[0] if len(tokens) == 1 else math.prod(tokens)
         if inplace:
             q_out, k_out = q, k
+            if k is not None and k.data_ptr() == q.data_ptr() and q.numel() and k.numel():
+                raise ValueError(f"{what}: in place on q and k that begin at one address")
             q_args = _in_place(what, q, T)
             k_args = _NO_TENSOR if k is None else _in_place(what, k, T)
         else:

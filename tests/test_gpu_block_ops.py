@@ -157,6 +157,9 @@ def test_attention_large_and_equal_scores(cuda_device):
     dev = cuda_device
     run_attention(cuda_device, [260], [700], 2, 1, 64, HF, seed=1, scale=2.0)
     run_attention(cuda_device, [3], [900], 8, 2, 128, seed=2, scale=-3.0, max_q=3)
+    for D in (64, 128, 256):   # negative and zero scales of a prompt: Q is negated in the product, every weight equal
+        run_attention(cuda_device, [300, 40], [700, 40], 4, 2, D, seed=3, scale=-0.5)
+        run_attention(cuda_device, [300, 40], [700, 40], 4, 2, D, HF, seed=4, scale=0.0)
     for nq in (2, 333):
         n = 700
         q = torch.full((nq, 2, 64), 0.5, dtype=BF, device=dev)
@@ -375,6 +378,25 @@ def test_rope_in_place_on_slices(cuda_device):
             yq, yk = rope(q, k, pos)
             rope(q, k, pos, inplace=True)
         assert torch.equal(q, yq) and torch.equal(k, yk) and torch.equal(base[:, 6 * D:], before[:, 6 * D:])
+
+
+def test_rope_refuses_in_place_overlaps_and_takes_empty_batches(cuda_device):
+    from onecomp_runtime.layers import RotaryEmbedding
+    dev = cuda_device
+    rope = RotaryEmbedding(64, device=dev)
+    q, pos = randn(dev, 5, 4, 64), torch.arange(5, device=dev)
+    with torch.no_grad():
+        for a, b in ((q, q), (q[:, :1].expand(5, 4, 64), None), (q, q[:, :2])):
+            with pytest.raises(ValueError):
+                rope(a, b, pos, inplace=True)
+        with pytest.raises(ValueError, match="tensors on"):
+            rope(q, None, pos.cpu())
+        e, k = rope(q[:0], q[:0, :2], pos[:0])
+        assert e.shape == (0, 4, 64) and k.shape == (0, 2, 64)
+        ee = rope(q[:0].view(0, 1, 4, 64), None, pos[:0].view(0, 1))[0]
+        assert ee.shape == (0, 1, 4, 64)
+        one = rope(q, None, torch.full((1,), 7, device=dev).expand(5))[0]      # one position for all tokens
+        assert torch.equal(one, rope(q, None, torch.full((5,), 7, device=dev))[0])
 
 
 def test_rope_leading_dimensions_and_axes(cuda_device):
