@@ -53,8 +53,8 @@ __device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report 
 }
 
 // One CTA's share of the rows that no sequence owns, in front of the first one and behind the last: zeros
-// (D is a multiple of 8, rows 16-byte aligned).
-__device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, int n_ctas) {
+// (D is a multiple of 8, rows 16-byte aligned). By `threads` threads of the CTA, of which this is `tid`.
+__device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, int n_ctas, int tid, int threads) {
   if (!p.cu_q) return;
   const int vecs = p.D / 8;
   const int head = p.B > 0 ? min(max(p.cu_q[0], 0), p.Tq) : 0;
@@ -62,7 +62,7 @@ __device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, 
   const long long rows = (long long)head + (p.Tq - tail);
   for (long long r = cta; r < rows; r += n_ctas) {
     const long long t = r < head ? r : tail + (r - head);
-    for (int i = threadIdx.x; i < p.Hq * vecs; i += blockDim.x)
+    for (int i = tid; i < p.Hq * vecs; i += threads)
       *reinterpret_cast<uint4*>(p.out + t * p.o_st + (i / vecs) * p.o_sh + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
   }
 }

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     total += sum;
   }
-  if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x);
+  if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
   const int n = (int)min(total, (long long)gridDim.x);   // CTAs with work
   if ((int)blockIdx.x >= n) return;
   long long u, u_end;

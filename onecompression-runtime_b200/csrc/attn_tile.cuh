@@ -103,14 +103,18 @@ struct TileWork {
   int nb[2];                             // blocks of each tile
 };
 
-// The sequence and first token of a token range; false behind the sequence's end.
+// The sequence and first token of a token range; false behind the sequence's end. A whole warp searches: its
+// lanes look at 32 places of the table at a time, one load's latency for up to 32 sequences.
 template <int DP> __device__ __forceinline__ bool tile_range(const AttnParams& p, const TileGrid& tg, int slot, TileWork& w) {
   const int R = TileCfg<DP>::kTiles * tg.tokens;
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    const int q0 = p.cu_q ? min(max(p.cu_q[mid], 0), p.Tq) : 0;
-    if (q0 / R + mid <= slot) lo = mid; else hi = mid;
+  int lo = 0, n = p.B;   // the last sequence of [lo, lo + n) that starts at or before the slot
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lane_id() * step;
+    const bool before = at < n && (p.cu_q ? min(max(p.cu_q[lo + at], 0), p.Tq) : 0) / R + lo + at <= slot;
+    const unsigned mask = __ballot_sync(0xffffffffu, before);
+    const int k = mask ? 31 - __clz(mask) : 0;
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   w.s = attn_seq(p, lo);
   const long long t0 = (long long)(slot - (w.s.q0 / R + lo)) * R;
@@ -173,11 +177,14 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   volatile int* odd_values = abort_flag + 1;   // an infinity or NaN was taken out of a V block
   const int warp = warp_uniform(warp_id()), lane = lane_id();
 
-  if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x);
+  TileWork w;
+  const bool work = tile_work<DP>(p, tg, w);
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += Cfg::kThreads) attn_seq(p, b, true);
-  TileWork w;
-  if (!tile_work<DP>(p, tg, w)) return;
+  if (!work) {
+    if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
+    return;
+  }
   const Seq s = w.s;
   const int off = s.nk - s.nq;   // the same for a part of the keys, counted from its first
 
@@ -346,6 +353,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     } else {
       // ------------------------------------------------------------ V blocks at the end of what rows see
       const int tid = threadIdx.x - (kAux + 2) * 32;
+      if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, tid, 64);
       for (int e = 0; w.e0 + e < w.nblk; ++e) {
         const int j = w.e0 + e;
         if (!mbar_wait(&edge_full[e], 0, abort_flag, kDevErrWEmpty)) break;
@@ -542,7 +550,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p,
   const int row = blockIdx.y * 32 + lane_id(), col = blockIdx.z * 64 + warp_id() * kV;
   const int kvh = unit / tg.slots;
   TileWork w;
-  if (row >= tg.tokens * p.G || !tile_range<DP>(p, tg, tg.slots - 1 - (unit - kvh * tg.slots), w)) return;
+  if (!tile_range<DP>(p, tg, tg.slots - 1 - (unit - kvh * tg.slots), w) || row >= tg.tokens * p.G) return;
   const int tok = w.t0 + t * tg.tokens + row / p.G;
   if (tok >= w.s.nq || col >= p.D) return;
   auto part = [&](int z) {
