@@ -298,7 +298,7 @@ int oc_b200_nvls_allreduce_rmsnorm_bf16(void* mc_ptr, int rows, int cols, const 
 
 /* ---- transformer-block operators beside the packed linears -------------------
  * No reference counterpart (the reference leaves them to torch). All are stream-ordered, allocate
- * nothing and run on the current device.
+ * nothing and run on the current device. Rows, sequences, heads and features are each below 2^30.
  *
  * Rotary positions. Tensors are [T, H, D] (dtype f16, bf16 or f32), token and head strides in
  * elements, unit stride inside a head; k may be absent (Hk = 0). The first R of D values (R even) are
@@ -317,8 +317,9 @@ int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t
  * 16-byte aligned, D a multiple of 8 up to 256. Sequence b: query rows cu_q[b] .. cu_q[b+1], key rows
  * from cu_k[b], kv_lens[b] of them (NULL: up to cu_k[b+1]); cu_q = cu_k = NULL: one sequence of all
  * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros.
- * Query rows outside every sequence stay as they were, or become zeros with zero_unowned. The tables are read on the device; values outside the tensors are clamped and set the
- * device error word. max_q (0: unknown) is a hint of the longest query run; it only picks a kernel.
+ * Query rows outside every sequence stay as they were, or become zeros with zero_unowned. The tables
+ * are read on the device; values outside the tensors are clamped and set the device error word. max_q
+ * (0: unknown) is a hint of the longest query run; it only picks a kernel.
  * workspace: oc_b200_attention_workspace bytes for the same sizes on the current device (may be 0), any
  * contents, 16-byte aligned, not shared by calls that may run at once. out must not overlap the inputs. */
 size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q);

@@ -102,15 +102,15 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
     total += sum;
   }
   if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
-  const int n = (int)min(total, (long long)gridDim.x);   // CTAs with work
-  if ((int)blockIdx.x >= n) return;
+  const int busy = (int)min(total, (long long)gridDim.x);   // CTAs with work
+  if ((int)blockIdx.x >= busy) return;
   long long u, u_end;
   if (total < (1ll << 22)) {   // the grid is below 2^10: 32-bit divisions
-    u = (unsigned)total * blockIdx.x / (unsigned)n;
-    u_end = (unsigned)total * (blockIdx.x + 1) / (unsigned)n;
+    u = (unsigned)total * blockIdx.x / (unsigned)busy;
+    u_end = (unsigned)total * (blockIdx.x + 1) / (unsigned)busy;
   } else {
-    u = total * blockIdx.x / n;
-    u_end = total * (blockIdx.x + 1) / n;
+    u = total * blockIdx.x / busy;
+    u_end = total * (blockIdx.x + 1) / busy;
   }
   int b = 0;
   long long seq_begin = 0;   // first unit of sequence b
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
     }
     if (!whole && blk0 == 0 && threadIdx.x == 0) {
       const long long last = seq_begin + (item + 1) * nblk - 1;   // the item's last unit
-      desc[1] = (int)(((last + 1) * n - 1) / total);              // the CTA that holds it
+      desc[1] = (int)(((last + 1) * busy - 1) / total);           // the CTA that holds it
       desc[2] = s.q0;
       desc[3] = kvh;
       *reinterpret_cast<long long*>(desc + 4) = row0;

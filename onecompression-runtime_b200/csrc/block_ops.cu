@@ -52,6 +52,10 @@ template <typename K> int check_registers(K kern, int threads, int needed, const
   return OC_OK;
 }
 
+// Rows, sequences, heads and features stay below 2^30, so that sums of two of them, and the last block of keys
+// or tile of rows that begins below a count, stay below 2^31.
+bool too_many(int n) { return n >= 1 << 30; }
+
 // ------------------------------------------------------------------ rotary positions
 template <int DT, int V, bool INTER>
 int launch_rope(const oc::RopeParams& p0, int sms, cudaStream_t stream) {
@@ -321,6 +325,7 @@ extern "C" int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_o
     return fail(OC_ERR_INVALID, "rope: T=%d Hq=%d Hk=%d D=%d R=%d (R even, at most D; D at most 1024)", T, Hq, Hk, D, R);
   if (!dtf(dtype)) return fail(OC_ERR_INVALID, "rope: dtype %d", dtype);
   if (Hq > 65535 || Hk > 65535) return fail(OC_ERR_INVALID, "rope: %d + %d heads", Hq, Hk);
+  if (too_many(T)) return fail(OC_ERR_INVALID, "rope: %d tokens", T);
   if (T == 0 || Hq + Hk == 0) return OC_OK;
   if ((Hq && (!q || !q_out)) || (Hk && (!k || !k_out)) || !positions || !turns)
     return fail(OC_ERR_INVALID, "rope: NULL pointer");
@@ -356,6 +361,7 @@ extern "C" int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_o
 
 extern "C" size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q) {
   if (Tq <= 0 || Tk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return 0;
+  if (too_many(Tq) || too_many(Tk) || too_many(B) || too_many(Hq)) return 0;
   int dev = 0;
   if (current_device(&dev)) return 0;
   return attn_plan(Tq, Tk, B, Hq, Hkv, D, max_q, sm_count(dev)).ws;
@@ -372,6 +378,8 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
     return fail(OC_ERR_INVALID, "attention: Tq=%d Tk=%d B=%d Hq=%d Hkv=%d (Hq a multiple of Hkv)", Tq, Tk, B, Hq, Hkv);
   if (D <= 0 || D > 256 || D % 8 != 0)
     return fail(OC_ERR_UNSUPPORTED, "attention: head size %d (a multiple of 8 up to 256)", D);
+  if (too_many(Tq) || too_many(Tk) || too_many(B) || too_many(Hq))
+    return fail(OC_ERR_INVALID, "attention: Tq=%d Tk=%d B=%d Hq=%d (below 2^30)", Tq, Tk, B, Hq);
   if ((cu_q == nullptr) != (cu_k == nullptr)) return fail(OC_ERR_INVALID, "attention: cu_q and cu_k come together");
   if (!cu_q && B != 1) return fail(OC_ERR_INVALID, "attention: B=%d without sequence tables", B);
   if (!std::isfinite(scale * 1.4426950408889634f)) return fail(OC_ERR_INVALID, "attention: scale %g", (double)scale);
@@ -425,6 +433,8 @@ extern "C" int oc_b200_dense_gemm(const void* x, int64_t ldx, const void* w, int
   if (!dt16(dtype)) return fail(OC_ERR_INVALID, "dense_gemm: dtype %d (f16 or bf16)", dtype);
   if (M < 0 || N < 0 || K <= 0 || K % 8 != 0)
     return fail(OC_ERR_INVALID, "dense_gemm: M=%d N=%d K=%d (K a multiple of 8)", M, N, K);
+  if (too_many(M) || too_many(N) || too_many(K))
+    return fail(OC_ERR_INVALID, "dense_gemm: M=%d N=%d K=%d (below 2^30)", M, N, K);
   if (act < OC_ACT_NONE || act > OC_ACT_RELU) return fail(OC_ERR_INVALID, "dense_gemm: act %d", act);
   if (bias && !dtf(bias_dtype)) return fail(OC_ERR_INVALID, "dense_gemm: bias dtype %d", bias_dtype);
   if (M == 0 || N == 0) return OC_OK;

@@ -133,10 +133,9 @@ __global__ void __launch_bounds__(kDsThreads)
     if (leader) tc_commit(done);
   }
   __syncwarp();
-  bool ok = true;
   float* acc = reinterpret_cast<float*>(smem);   // [BN tokens][128 features]
   if (warp < 4) {
-    ok = mbar_wait(done, 0, abort_flag, kDevErrAccFull);
+    mbar_wait(done, 0, abort_flag, kDevErrAccFull);
     tc_fence_after();
   }
   __syncthreads();   // the ring's loads and the MMAs that read it are done: the accumulator moves in

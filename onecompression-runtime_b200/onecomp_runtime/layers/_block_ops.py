@@ -8,6 +8,7 @@ import torch
 
 from .. import _lib
 
+MAX_COUNT = 2**30 - 1   # rows, heads and features of a call: the kernels count them, and their sums, in 32 bits
 _NOTHING = contextlib.nullcontext()
 
 

@@ -6,7 +6,7 @@ import math
 import torch
 
 from .. import _lib
-from ._block_ops import inference_only, on_device, one_device, overlap
+from ._block_ops import MAX_COUNT, inference_only, on_device, one_device, overlap
 
 
 def _rows(t: torch.Tensor, copy: bool = True) -> tuple[torch.Tensor, int, int, int] | None:
@@ -63,6 +63,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
     Tq, Hq, D = q.shape
     Tk, Hkv, _ = k.shape
+    if max(Tq, Tk, Hq) > MAX_COUNT:
+        raise ValueError(f"{what}: {Tq} query rows, {Tk} key rows, {Hq} heads (each below 2**30)")
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} key heads")
     if D == 0 or D % 8 or D > 256:

@@ -3,10 +3,9 @@ checkpoint that are not packed (or that ``build_eager`` dequantized)."""
 from __future__ import annotations
 
 import torch
-import torch.nn.functional as F
 
 from .. import _lib
-from ._block_ops import inference_only, on_device, one_device, overlap
+from ._block_ops import MAX_COUNT, inference_only, on_device, one_device, overlap
 
 ACTIVATIONS = {None: 0, "none": 0, "gelu_tanh": 1, "gelu": 2, "silu": 3, "relu": 4}
 
@@ -58,6 +57,9 @@ def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
     N, K = weight.shape
+    M = x.numel() // max(K, 1)
+    if max(M, N, K) > MAX_COUNT:
+        raise ValueError(f"{what}: {M} rows, {N} x {K} weights (each below 2**30)")
     if K == 0 or K % 8:
         raise ValueError(f"{what}: K={K} must be a multiple of 8")
     if x.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != x.dtype:
@@ -73,7 +75,6 @@ def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     inference_only(what, x, weight, bias, residual, out)
     dev = one_device(what, x, weight, bias, residual, out)
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    M = x2.shape[0]
     res2 = residual if residual is None or residual.dim() == 2 else residual.reshape(M, N)
     if out is None:
         target = torch.empty(shape, dtype=x.dtype, device=dev)

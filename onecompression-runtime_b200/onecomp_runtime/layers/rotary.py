@@ -7,7 +7,7 @@ import math
 import torch
 
 from .. import _lib
-from ._block_ops import inference_only, on_device, one_device
+from ._block_ops import MAX_COUNT, inference_only, on_device, one_device
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None
@@ -183,9 +183,11 @@ class RotaryEmbedding(torch.nn.Module):
         if dtype not in _lib.DT or (k is not None and k.dtype is not dtype):
             raise TypeError(f"{what} takes fp16, bf16 or fp32 of one dtype, got {dtype} and "
                             f"{None if k is None else k.dtype}")
+        T = q_shape[0] if len(tokens) == 1 else math.prod(tokens)
+        if max(T, q_shape[-2], 0 if k is None else k.shape[-2]) > MAX_COUNT:
+            raise ValueError(f"{what}: {T} tokens, {q_shape[-2]} query heads (each below 2**30)")
         inference_only(what, q, k)
         dev = one_device(what, q, k, positions)
-        T = q_shape[0] if len(tokens) == 1 else math.prod(tokens)
         if inplace:
             q_out, k_out = q, k
             if k is not None and k.data_ptr() == q.data_ptr() and q.numel() and k.numel():

@@ -160,3 +160,32 @@ def test_c_entry_points_refuse_before_any_launch():
                dict(res=p, ldr=39)):
         assert dense(**kw) == 1, kw
     assert dense(M=0) == 0 and dense(N=0) == 0
+
+
+def test_counts_beyond_the_kernels_integers_are_refused():
+    """A count that 32 bits would cut (2^32 + 4 would run as 4 rows) is refused by the layers and by the C ABI."""
+    from onecomp_runtime import _lib
+    from onecomp_runtime.layers import RotaryEmbedding, linear_fused, packed_attention
+    a, many = q(3, 2, 8), 2**32 + 4
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        packed_attention(q(1, 2, 8).expand(many, 2, 8), a, a)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        packed_attention(a, q(1, 2, 8).expand(many, 2, 8), q(1, 2, 8).expand(many, 2, 8))
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        linear_fused(q(1, 8).expand(many, 8), q(40, 8))
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        linear_fused(q(3, 8), q(1, 8).expand(many, 8))
+    pos = torch.zeros(1, dtype=torch.int64).expand(many)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        RotaryEmbedding(8)(q(1, 1, 8).expand(many, 1, 8), None, pos)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        RotaryEmbedding(8)(q(1, 1, 8).expand(1, many, 8), None, pos[:1])
+
+    lib, p, big = _lib.lib(), ctypes.c_void_p(0x10000), 1 << 30
+    assert lib.oc_b200_rope(p, 8, 8, p, 8, 8, 1, None, 0, 0, None, 0, 0, 0, 1, big, 8, 8, p, 1, 1, p, None, 1.0, 0,
+                            None) == 1
+    for Tq, Tk, B, H in ((big, 4, 1, 1), (4, big, 1, 1), (4, 4, big, 1), (4, 4, 1, big)):
+        assert lib.oc_b200_attention(p, 8, 8, p, 8, 8, p, 8, 8, p, 8, 8, 1, Tq, Tk, H, H, 8, p, p, None, B, 1, 0.1, 0, 0, p,
+                                     0, None) == 1
+    for M, N, K in ((big, 8, 8), (4, big, 8), (4, 8, big)):
+        assert lib.oc_b200_dense_gemm(p, big, p, big, 1, M, N, K, None, 0, None, 0, 0, p, big, None) == 1
