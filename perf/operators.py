@@ -5,27 +5,14 @@ over packed sequences, and the dense 16-bit linear with its epilogue.
 ``onecomp_runtime``. Sizes follow the framework's own workloads: 32 heads of 128 (hidden 4096, fc1 16384)
 of the video-DiT stack, the 5120-wide decode layers; wide heads rotated in part are the other common form.
 """
-import functools
 import math
 import random
-import sys
-from pathlib import Path
 
 import torch
 
 own = False
 
 _DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
-
-
-@functools.lru_cache(maxsize=None)
-def _layers():
-    """The framework's layers, imported once; the package lies one folder below the repository's root."""
-    root = str(Path(__file__).resolve().parents[1] / "onecompression-runtime_b200")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from onecomp_runtime import layers
-    return layers
 
 
 # ------------------------------------------------------------------------------------------- cases
@@ -165,8 +152,9 @@ def prepare(case, seed):
                   k=qkv[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d)),
                   pos=torch.randint(0, case["far"], shape, generator=g, device=dev, dtype=torch.int64))
         if own:
-            st["rope"] = _layers().RotaryEmbedding(d, rotary_dim=case["rot"], layout=case["layout"], axes=axes,
-                                                   scaling=_rope_scaling(case), device=dev)
+            from onecomp_runtime.layers import RotaryEmbedding
+            st["rope"] = RotaryEmbedding(d, rotary_dim=case["rot"], layout=case["layout"], axes=axes,
+                                         scaling=_rope_scaling(case), device=dev)
         else:
             freq, gain = _frequencies(case, axes)
             st["freq"], st["gain"] = torch.tensor(freq, dtype=torch.float64, device=dev), gain
@@ -198,7 +186,7 @@ def run(state):
 
 
 def _run_own(op, st):
-    layers = _layers()
+    from onecomp_runtime import layers
     if op in ("decode", "prompt"):
         return layers.packed_attention(st["q"], st["k"], st["v"], st["cu_q"], st["cu_k"], kv_lens=st.get("kv_lens"),
                                        causal=st["case"].get("causal", True), max_seqlen_q=st["max_q"])
