@@ -323,7 +323,10 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         return true;
       };
       // S(j + 1) overwrites the columns of P(j) (two tiles) or P(j - 1) (one tile): only once the
-      // product that reads them is done
+      // product that reads them is done. Where P has columns of its own (head size 64) the product before
+      // is waited for instead. A wait by parity tells a phase from the one before it only, so every wait on
+      // pv_done needs the knowledge that the phase before is over and that the one behind it cannot be:
+      // this warp sees phase j - 1 before it issues PV(j), and S(j + 1), issued later, carries that to the softmax.
       auto pv_over = [&](const int t, const int j) {
         return mbar_wait_warp(&pv_done[t], j & 1, abort_flag, kDevErrAccFull);
       };
@@ -332,10 +335,10 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         if (ok && nb0 > 0) ok = qk(0, 0, true);
         if (ok && last_tile && nblk > 0) ok = qk(1, 0, nb0 == 0);
         for (int j = 0; ok && j < nblk; ++j) {
-          if (j < nb0) ok = pv(0, j, true);
+          if (j < nb0) ok = (DP != 64 || j == 0 || pv_over(0, j - 1)) && pv(0, j, true);
           if (ok && j + 1 < nb0) ok = (DP == 64 || pv_over(0, j)) && qk(0, j + 1, true);
           if (!last_tile) continue;
-          if (ok) ok = pv(1, j, j >= nb0);
+          if (ok) ok = (DP != 64 || j == 0 || pv_over(1, j - 1)) && pv(1, j, j >= nb0);
           if (ok && j + 1 < nblk) ok = (DP == 64 || pv_over(1, j)) && qk(1, j + 1, j + 1 >= nb0);
         }
       } else {
@@ -468,6 +471,10 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
         if (c >= 2) {   // 96 keys' weights: the product starts; then the rest
           tc_wait_st();
           tc_fence_before();
+          // The last product starts with this arrival: the one before it is seen to be done first, or its phase
+          // of pv_done could pass for the last one's below, or be over before it is looked at.
+          if (c == 3 && j > 0 && j == nb - 1)
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (j - 1) & 1, abort_flag, kDevErrAccEmpty));
           mbar_arrive(c == 3 ? &p_full[b] : &p_part[b]);
         }
       }
@@ -475,9 +482,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       f2_unpack(sum, s0, s1);
       l += s0 + s1;
     }
-    // the row's output. With one tile the last S was ready before the product before last was: that
-    // one is waited for first, or its phase would pass for the last one's.
-    if (!kTwo && ok && nb > 1) ok = mbar_wait(&pv_done[t], (nb - 2) & 1, abort_flag, kDevErrAccEmpty);
+    // the row's output
     if (ok && nb > 0) ok = mbar_wait(&pv_done[t], (nb - 1) & 1, abort_flag, kDevErrAccEmpty);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
