@@ -5,6 +5,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -13,12 +14,17 @@ _NOTHING = contextlib.nullcontext()
 
 
 def inference_only(what: str, *tensors: torch.Tensor | None) -> None:
-    """The operators have no backward pass: refuse inputs that autograd would track."""
+    """The operators have no derivatives: refuse inputs that autograd would track, backward or forward."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} is inference only (no backward pass): call it under torch.no_grad() or "
                                    "detach the inputs")
+    if forward_ad._current_level >= 0:   # inside a dual_level block; asking every tensor would cost 4 us a call
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} is inference only (no forward-mode derivative): pass the primals "
+                                   "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def one_device(what: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
