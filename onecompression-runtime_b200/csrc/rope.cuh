@@ -2,10 +2,11 @@
 //   y1 = g (x1 cos a - x2 sin a),  y2 = g (x2 cos a + x1 sin a),  a = position * f_pair.
 //
 // Angles: f_pair is kept as the fraction of a turn per position, a 0.64 fixed-point number, so
-// position * fraction modulo 2^64 (one integer product, wrapping) is the angle modulo one turn,
-// exact for every 64-bit position, negative ones included. Its upper 32 bits as a signed number are
-// the angle in half turns x 2^31, which sincospif takes without a range reduction; the error is
-// 2^-25 of a half turn at any position, where an fp32 product would lose the angle of far positions.
+// position * fraction modulo 2^64 (one integer product, wrapping) is the angle modulo one turn, for
+// every 64-bit position, negative ones included. Its upper 32 bits as a signed number are the angle in
+// half turns x 2^31, which sincospif takes without a range reduction. The error is 2^-25 of a half turn
+// (the conversion to fp32) plus the position times what the table is off (2^-64 of a half turn at least);
+// an fp32 product would lose the angle of far positions.
 //
 // Bound by HBM: each value is read and written once. A block takes TB tokens, computes their
 // TB * R/2 sines and cosines once into shared memory (all heads of a token share them) and then

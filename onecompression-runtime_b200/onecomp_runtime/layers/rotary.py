@@ -103,7 +103,8 @@ class RotaryEmbedding(torch.nn.Module):
     :func:`rotary_frequencies` (not with ``axes``); ``inv_freq``: frequencies of the pairs, instead of base
     and scaling.
 
-    Angles are exact modulo one turn for every integer position (64-bit fixed point), however far.
+    Angles are 64-bit fixed point modulo one turn, for any integer position: off by 2^-25 of a half turn, plus
+    position times the table's rounding (2^-52 of the frequency, as doubles have it, and 2^-64 of a half turn).
     The module has no buffers, so it survives a build on the meta device; the table of a device is copied
     there by the first call on it (or by ``device=``), which belongs before a graph capture.
     """

@@ -33,3 +33,34 @@ def test_forward_mode_derivatives_are_refused():
         for call in (lambda: packed_attention(a, a, primal), lambda: rope(a, primal, pos), lambda: linear_fused(x, w)):
             with pytest.raises(RuntimeError, match="CUDA"):
                 call()
+
+
+def pi_by_machin(digits: int):
+    """pi as a fraction, from 16 atan(1/5) - 4 atan(1/239), to this many decimals."""
+    from fractions import Fraction
+
+    def atan_inverse(n):
+        total, k = Fraction(0), 0
+        while n ** (2 * k + 1) < 10 ** (digits + 5):
+            total += Fraction((-1) ** k, (2 * k + 1) * n ** (2 * k + 1))
+            k += 1
+        return total
+
+    return 16 * atan_inverse(5) - 4 * atan_inverse(239)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(base=1e6), dict(scaling={"type": "ntk", "factor": 8.0}),
+                                dict(scaling={"type": "yarn", "factor": 16.0, "original_max_position": 32768}),
+                                dict(inv_freq=[1.0, 3.0, -1.0, 0.75, 6.25, -1e-9, 123.456, 0.0] * 4)])
+def test_rotary_table_against_long_arithmetic(kw):
+    """A fraction of a turn is off by 2^-52 of itself before it is taken modulo one turn: division and 2 pi are each
+    rounded to a double (2^-53 and 2^-54 relative), and to a unit of 2^-64."""
+    from fractions import Fraction
+    from onecomp_runtime.layers import RotaryEmbedding
+    two_pi = 2 * pi_by_machin(50)
+    rope = RotaryEmbedding(64, **kw)
+    for f, t in zip(rope.inv_freq, rope._turns):
+        exact = Fraction(f) / two_pi
+        off = (t - exact * 2**64) % 2**64
+        assert min(off, 2**64 - off) <= abs(exact) * 2**12 + 1, (f, float(off))
+        assert -2**63 <= t < 2**63

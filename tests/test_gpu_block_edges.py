@@ -55,3 +55,30 @@ def test_attention_products_done_before_they_are_read(cuda_device, D, grows):
             with torch.no_grad():
                 ref.check(packed_attention(q, k, v, c, c, causal=causal, max_seqlen_q=1100), want, tol, f"D={D}")
     assert error_word(dev) == 0
+
+
+# ---------------------------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
+def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
+    """Positions up to 2^50, against angles in fractions with a pi of 50 digits. Beside the bound of the near
+    positions (its sine and cosine hold 2^-25 of a half turn) the table counts: a fraction of a turn is off by 2^-52 of
+    itself and, rounded to a unit of 2^-64 turns, by half of that (pi 2^-64 as an angle), times the position."""
+    from fractions import Fraction
+    from test_block_edges_cpu import pi_by_machin
+    from onecomp_runtime.layers import RotaryEmbedding
+    dev = cuda_device
+    rope = RotaryEmbedding(64, scaling=scaling)
+    where = [2**31, -2**31, 2**33 + 12345, 2**40 + 1, 2**45 - 7, 2**50 + 3, -2**50]
+    pi = pi_by_machin(50)
+    turn = [[float((Fraction(f) * p / (2 * pi)) % 1) for f in rope.inv_freq] for p in where]
+    ang = torch.tensor(turn, dtype=torch.float64, device=dev) * (2 * math.pi)
+    q = randn(dev, len(where), 5, 64, dtype=torch.float32, seed=6)
+    with torch.no_grad():
+        y, _ = rope(q, None, torch.tensor(where, device=dev))
+    want, tol = ref.rope(q, ang, rope.gain, 64, False)
+    mag = q.double()[..., :32].abs() + q.double()[..., 32:].abs()
+    far = torch.tensor([[abs(p) * (abs(f) * 2.0 ** -52 + math.pi * 2.0 ** -64) for f in rope.inv_freq] for p in where],
+                       dtype=torch.float64, device=dev)
+    mag = mag * far.unsqueeze(1)
+    tol = tol + torch.cat([mag, mag], -1)
+    ref.check(y, want, tol, "far positions")
