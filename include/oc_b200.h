@@ -316,7 +316,8 @@ int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t
  * [Tq, Hq, D]; k, v: [Tk, Hkv, D]; token and head strides in elements, multiples of 8, tensors
  * 16-byte aligned, D a multiple of 8 up to 256. Sequence b: query rows cu_q[b] .. cu_q[b+1], key rows
  * from cu_k[b], kv_lens[b] of them (NULL: up to cu_k[b+1]); cu_q = cu_k = NULL: one sequence of all
- * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros.
+ * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros, one whose
+ * visible scores are all minus infinity NaN.
  * Query rows outside every sequence stay as they were, or become zeros with zero_unowned. The tables
  * are read on the device; values outside the tensors are clamped and set the device error word. max_q
  * (0: unknown) is a hint of the longest query run; it only picks a kernel.

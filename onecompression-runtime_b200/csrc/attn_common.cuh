@@ -2,7 +2,8 @@
 //
 // Sequence b owns the query rows [cu_q[b], cu_q[b+1]) and the key rows that start at cu_k[b]; it
 // sees kv_lens[b] of them, or all up to cu_k[b+1]. With causal masking the last query sees the last
-// key: query i of nq sees the keys j <= i + nk - nq. A row that sees no key gives zeros.
+// key: query i of nq sees the keys j <= i + nk - nq. A row that sees no key gives zeros; a row whose
+// visible scores are all minus infinity gives NaN, as its softmax does.
 // The tables live on the device and are clamped to the tensors here, so no table value can send an
 // access out of range; a clamped value sets the device error word.
 #pragma once
@@ -30,6 +31,16 @@ struct AttnParams {
 };
 
 struct Seq { int q0, nq, k0, nk; };
+
+// The first token of a sequence that sees a key (nq where none does).
+__device__ __forceinline__ int attn_first_seeing(const AttnParams& p, const Seq& s) {
+  return p.causal ? max(0, s.nq - s.nk) : s.nk > 0 ? 0 : s.nq;
+}
+// What the sum of weighted values is multiplied with, from the sum of weights. The key with the largest score
+// weighs at least 1, so a sum of zero means no key, or no score above minus infinity.
+__device__ __forceinline__ float attn_inverse(float l, bool sees_keys) {
+  return l > 0.f ? 1.f / l : l == 0.f ? (sees_keys ? __int_as_float(0x7fffffff) : 0.f) : l;
+}
 
 __device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report = false) {
   int q0 = 0, q1 = p.Tq, k0 = 0, k1 = p.Tk;

@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
       }
       if (whole) {
         if (c4 < p.D) {
-          const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
           const long long row = row0 + r;
+          const float inv = attn_inverse(lsum, row / p.G >= attn_first_seeing(p, s));
           uint16_t* dst = p.out + (s.q0 + row / p.G) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + c4;
           *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_rn<BF16>(acc.x * inv, acc.y * inv),
                                                       pack2_rn<BF16>(acc.z * inv, acc.w * inv));
@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
       desc[2] = s.q0;
       desc[3] = kvh;
       *reinterpret_cast<long long*>(desc + 4) = row0;
+      desc[6] = attn_first_seeing(p, s);
       desc[0] = rows;
     }
     __syncthreads();
@@ -458,8 +459,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParam
     f[i] = ex2(sm_m[row_in][i] - ref);
     total += f[i] * sm_l[row_in][i];
   }
-  const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
   const long long row = *reinterpret_cast<const long long*>(desc + 4) + r;
+  const float inv = attn_inverse(total, row / p.G >= desc[6]);
   uint16_t* dst = p.out + (desc[2] + row / p.G) * p.o_st + (desc[3] * p.G + row % p.G) * p.o_sh + lane * kV;
   if (lane * kV < p.D) {
 #pragma unroll

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
       tc_fence_after();
       const bool odd = *odd_values != 0;
       const bool direct = tg.splits == 1;
-      const float inv = !direct ? 1.f : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const float inv = direct ? attn_inverse(l, limit >= 0) : 1.f;
       uint16_t* dst = p.out + (long long)(s.q0 + tok) * p.o_st + head * p.o_sh;
       float* part = direct ? nullptr : tg.part + ((long long)blockIdx.x * Cfg::kTiles + t) * (128 * (DP + 2)) + row;
 #pragma unroll 1
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p,
 #pragma unroll
     for (int i = 0; i < kV; ++i) acc[i] += f * x[(col + i) * 128];
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = attn_inverse(l, tok >= attn_first_seeing(p, w.s));
   uint16_t* dst = p.out + (long long)(w.s.q0 + tok) * p.o_st + (kvh * p.G + row % p.G) * p.o_sh + col;
   *reinterpret_cast<uint4*>(dst) =
       make_uint4(pack2_rn<BF16>(acc[0] * inv, acc[1] * inv), pack2_rn<BF16>(acc[2] * inv, acc[3] * inv),

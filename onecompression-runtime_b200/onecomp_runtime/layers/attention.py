@@ -48,7 +48,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     device error word (``_lib.read_device_error``).
 
     ``causal``: the last query of a sequence sees its last key, query i of nq the keys up to
-    ``i + nk - nq``. Rows that see no key give zeros; what lies behind a sequence's keys never reaches a
+    ``i + nk - nq``. Rows that see no key give zeros (rows whose visible scores are all minus infinity give NaN, as
+    their softmax does); what lies behind a sequence's keys never reaches a
     result, not even infinities or NaN. ``scale`` defaults to ``D ** -0.5``. ``max_seqlen_q``: the longest
     query run if the host knows it; it only helps to pick the kernel (results are right whatever it says),
     and matters where one batch holds prompts beside single tokens: the mean run counts without it.

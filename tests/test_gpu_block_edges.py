@@ -57,6 +57,33 @@ def test_attention_products_done_before_they_are_read(cuda_device, D, grows):
     assert error_word(dev) == 0
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("case", [([3], [3]), ([1], [2000]), ([5], [3]), ([200], [200]), ([40], [3000]), ([300, 2], [150, 2])])
+def test_attention_rows_of_minus_infinity(cuda_device, D, case):
+    """A row that sees keys, all with scores of minus infinity, is NaN, as its softmax is; a row that sees no key is
+    zero; one finite score is enough for a finite row. Few rows, prompts, and keys split over CTAs."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    lq, lk = case
+    q, k, v = (randn(dev, sum(n), h, D, seed=i) for i, (n, h) in enumerate(((lq, 4), (lk, 2), (lk, 2))))
+    q[..., 0] = q[..., 0].abs() + 1
+    k[..., 0] = -math.inf
+    finite = k.clone()
+    finite[0, :, 0] = 1.0                       # the first key of the first sequence
+    for causal in (True, False):
+        sees = torch.cat([torch.arange(a, device=dev) + (b - a if causal else b) >= 0 for a, b in zip(lq, lk)])
+        with torch.no_grad():
+            o = packed_attention(q, k, v, starts(dev, lq), starts(dev, lk), causal=causal, max_seqlen_q=max(lq))
+            f = packed_attention(q, finite, v, starts(dev, lq), starts(dev, lk), causal=causal, max_seqlen_q=max(lq))
+        assert bool(torch.isnan(o[sees]).all()) and bool((o[~sees] == 0).all())
+        first = v[:1].repeat_interleave(2, 1)   # a weight of one on the first key
+        here = sees.clone()
+        here[lq[0]:] = False
+        assert bool((f[here] == first).all()) and bool((f[:lq[0]][~sees[:lq[0]]] == 0).all())
+        assert bool(torch.isnan(f[lq[0]:]).all())
+    assert error_word(dev) == 0
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
