@@ -33,6 +33,7 @@ namespace oc {
 constexpr int kTileKeys = 128;
 constexpr int kTileUnitBytes = 128 * 128;   // [128 rows x 64 columns] of 16-bit values
 constexpr int kTileMaxEdges = 3;
+constexpr int kTileNegate = 1, kTileZeroScale = 2;   // of a negative and a zero softmax scale
 template <int DP> struct TileCfg {
   static constexpr int kTiles = DP == 256 ? 1 : 2;          // row tiles of a CTA
   static constexpr int kRows = kTiles * 128;
@@ -154,7 +155,7 @@ template <int DP> __device__ __forceinline__ int v_use(int j, int nblk) {
 
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
-    attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const TileGrid tg, const int negate) {
+    attn_tile_kernel(const __grid_constant__ TileMaps maps, const AttnParams p, const TileGrid tg, const int mode) {
   using Cfg = TileCfg<DP>;
   constexpr int U = Cfg::kUnits, GU = Cfg::kGroup, GN = Cfg::kGroups, NB = Cfg::kSlots * GN;
   constexpr bool kTwo = Cfg::kTiles == 2;
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     } else if (warp == kAux + 1) {
       // ------------------------------------------------------------ MMA
       // The whole warp runs this with warp-uniform values; one elected thread issues.
-      const uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128) | (negate ? 1u << 13 : 0u);
+      const uint32_t idesc_qk = make_idesc_f16(BF16, 128, 128) | (mode & kTileNegate ? 1u << 13 : 0u);
       constexpr uint32_t idesc_pv = make_idesc_f16(BF16, 128, DP) | (1u << 16);   // B is MN-major
       const int last_tile = warp_uniform(w.ntile - 1), nblk = warp_uniform(w.nblk), e0 = warp_uniform(w.e0);
       const int nb0 = warp_uniform(w.nb[0]);
@@ -409,6 +410,12 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tmem + lanes + Cfg::s_col(b) + c * 32, v[c]);
       tc_wait_ld();
+      if (mode & kTileZeroScale) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c][i] = __float_as_uint(__uint_as_float(v[c][i]) * 0.f);
+      }
       const bool edge = j * kTileKeys + kTileKeys - 1 > limit0;   // some row of the warp does not see all
       if (edge) {
         const int seen = limit - j * kTileKeys;

@@ -168,10 +168,10 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, const oc::TileGri
   if (int rc = attn_tmap(&maps.v, BF16, p.v, p.D, p.Hkv, p.Tk, p.v_sh, p.v_st, 1, oc::kTileKeys)) return rc;
   const long long units = (long long)tg.slots * p.Hkv;
   if (units * tg.splits > INT_MAX / 2) return fail(OC_ERR_INVALID, "attention: %lld token ranges", units);
-  // the softmax takes its maximum before the scale: a negative scale negates Q in the product, and
-  // zero becomes a scale that rounds every finite score to zero but leaves masked ones infinite
-  const int negate = p.scale_log2 < 0.f;
-  p.scale_log2 = std::fmax(std::fabs(p.scale_log2), 1e-30f);
+  // The softmax takes its maximum before the scale: a negative scale negates Q in the product. A scale of
+  // zero makes every finite score zero there and every other NaN, and a scale of one keeps them so.
+  const int mode = (p.scale_log2 < 0.f ? oc::kTileNegate : 0) | (p.scale_log2 == 0.f ? oc::kTileZeroScale : 0);
+  p.scale_log2 = mode & oc::kTileZeroScale ? 1.f : std::fabs(p.scale_log2);
   auto kern = oc::attn_tile_kernel<BF16, DP>;
   static const int regs_rc = check_registers(
       kern, Cfg::kThreads, Cfg::kTiles == 2 ? Cfg::kSoftmaxThreads * Cfg::kSoftmaxRegs + 128 * Cfg::kAuxRegs : 0,
@@ -179,7 +179,7 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, const oc::TileGri
   if (regs_rc) return fail(regs_rc, "attention (tile): register count of the build");
   static std::atomic<uint64_t> smem_set{0};
   if (int rc = set_smem(kern, Cfg::kSmem, smem_set)) return rc;
-  kern<<<(unsigned)(units * tg.splits), Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, tg, negate);
+  kern<<<(unsigned)(units * tg.splits), Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, tg, mode);
   if (int rc = launch_check("attention (tile)")) return rc;
   if (tg.splits == 1) return OC_OK;
   return launch_pdl(oc::attn_tile_join_kernel<BF16, DP>, dim3((unsigned)(units * Cfg::kTiles), 4, DP / 64), dim3(256), 0, stream,

@@ -84,6 +84,28 @@ def test_attention_rows_of_minus_infinity(cuda_device, D, case):
     assert error_word(dev) == 0
 
 
+@pytest.mark.parametrize("nq", [3, 200])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_zero_and_tiny_scales(cuda_device, nq, D):
+    """A scale of zero weighs every visible key alike, whatever the scores' size (infinite ones give NaN), and a tiny
+    scale still tells scores apart that are large enough."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    nk = 500
+    q, k, v = randn(dev, nq, 4, D, seed=1, std=1e14), randn(dev, nk, 2, D, seed=2, std=1e15), randn(dev, nk, 2, D, seed=3)
+    with torch.no_grad():
+        for causal in (True, False):
+            o = packed_attention(q, k, v, causal=causal, scale=0.0)
+            ref.check(o, *ref.attention(q, k, v, [(0, nq, 0, nk)], causal, 0.0), "scale zero")
+            for scale in (1e-30, -3e-31):
+                o = packed_attention(q, k, v, causal=causal, scale=scale)
+                ref.check(o, *ref.attention(q, k, v, [(0, nq, 0, nk)], causal, scale), f"scale {scale}")
+            big = k.clone()
+            big[7] = math.inf                        # q . k is infinite or NaN: times zero it is NaN
+            assert bool(torch.isnan(packed_attention(q, big, v, causal=causal, scale=0.0)).all())
+    assert error_word(dev) == 0
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
