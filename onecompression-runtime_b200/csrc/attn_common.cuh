@@ -69,7 +69,7 @@ __device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, 
   if (!p.cu_q) return;
   const int vecs = p.D / 8;
   const int head = p.B > 0 ? min(max(p.cu_q[0], 0), p.Tq) : 0;
-  const int tail = min(max(p.cu_q[p.B], head), p.Tq);
+  const int tail = p.B > 0 ? min(max(p.cu_q[p.B], head), p.Tq) : 0;   // without sequences every row is
   const long long rows = (long long)head + (p.Tq - tail);
   for (long long r = cta; r < rows; r += n_ctas) {
     const long long t = r < head ? r : tail + (r - head);

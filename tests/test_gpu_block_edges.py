@@ -106,6 +106,29 @@ def test_attention_zero_and_tiny_scales(cuda_device, nq, D):
     assert error_word(dev) == 0
 
 
+def dirty(dev, t):
+    """Leave NaN in the block that the allocator hands to the next tensor of this size."""
+    junk = torch.full_like(t, math.nan, memory_format=torch.contiguous_format)
+    torch.cuda.synchronize(dev)
+    del junk
+
+
+@pytest.mark.parametrize("first", [0, 2, 5, 9])
+def test_attention_without_sequences_is_zero_everywhere(cuda_device, first):
+    """Tables of one entry hold no sequence, whatever the entry says: a new output is all zeros, a given one stays."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    q = randn(dev, 5, 4, 64)
+    with torch.no_grad():
+        dirty(dev, q)
+        o = packed_attention(q, q, q, table(dev, first), table(dev, first))
+        assert bool((o == 0).all())
+        kept = torch.full_like(q, 3.0)
+        packed_attention(q, q, q, table(dev, first), table(dev, first), out=kept)
+        assert bool((kept == 3).all())
+    error_word(dev)
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
