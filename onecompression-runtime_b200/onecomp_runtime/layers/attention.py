@@ -76,10 +76,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if (cu_seqlens_q is None) != (cu_seqlens_k is None):
         raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k come together")
     B = 1 if cu_seqlens_q is None else cu_seqlens_q.numel() - 1
+    if B < 0:
+        raise ValueError(f"{what}: cu_seqlens_q must be int32 [sequences + 1], got an empty tensor")
     for name, t, n in (("cu_seqlens_q", cu_seqlens_q, B + 1), ("cu_seqlens_k", cu_seqlens_k, B + 1),
                        ("kv_lens", kv_lens, B)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or n < 1):
-            raise ValueError(f"{what}: {name} must be int32 [{max(n, 1)}], got {t.dtype} {tuple(t.shape)}")
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n):
+            raise ValueError(f"{what}: {name} must be int32 [{n}], got {t.dtype} {tuple(t.shape)}")
     scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what}: scale {scale}")

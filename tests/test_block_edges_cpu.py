@@ -64,3 +64,18 @@ def test_rotary_table_against_long_arithmetic(kw):
         off = (t - exact * 2**64) % 2**64
         assert min(off, 2**64 - off) <= abs(exact) * 2**12 + 1, (f, float(off))
         assert -2**63 <= t < 2**63
+
+
+def test_attention_takes_the_lengths_of_an_empty_batch():
+    """No sequence: the tables hold one entry and kv_lens none. Past the checks such a call ends here in the refusal
+    of CPU tensors; wrong sizes and empty tables are refused before."""
+    from onecomp_runtime.layers import packed_attention
+    a, one, none = zeros(3, 4, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        packed_attention(a, a, a, one, one, kv_lens=none)
+    with pytest.raises(ValueError, match="kv_lens"):
+        packed_attention(a, a, a, one, one, kv_lens=one)
+    with pytest.raises(ValueError, match="cu_seqlens_q"):
+        packed_attention(a, a, a, none, none)
+    with pytest.raises(ValueError, match="cu_seqlens_q"):
+        packed_attention(a, a, a, none, one, kv_lens=none)

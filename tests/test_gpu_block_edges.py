@@ -129,6 +129,16 @@ def test_attention_without_sequences_is_zero_everywhere(cuda_device, first):
     error_word(dev)
 
 
+def test_attention_of_an_empty_batch_with_lengths(cuda_device):
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    q, none = randn(dev, 5, 4, 64), torch.zeros(0, dtype=torch.int32, device=dev)
+    with torch.no_grad():
+        assert bool((packed_attention(q, q, q, table(dev, 0), table(dev, 0), kv_lens=none) == 0).all())
+        e = packed_attention(q[:0], q, q, table(dev, 0), table(dev, 0), kv_lens=none)
+    assert e.shape == (0, 4, 64) and error_word(dev) == 0
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
