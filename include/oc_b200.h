@@ -319,8 +319,9 @@ int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t
  * rows (B = 1). causal: query i of nq sees keys 0 .. i + nk - nq. A row that sees no key gives zeros, one whose
  * visible scores are all minus infinity NaN.
  * Query rows outside every sequence stay as they were, or become zeros with zero_unowned. The tables
- * are read on the device; values outside the tensors are clamped and set the device error word. max_q
- * (0: unknown) is a hint of the longest query run; it only picks a kernel.
+ * are read on the device; values outside the tensors are clamped and set the device error word; a cu_q that
+ * decreases sets it and runs no sequence (no row is owned). max_q (0: unknown) is a hint of the longest
+ * query run; it only picks a kernel.
  * workspace: oc_b200_attention_workspace bytes for the same sizes on the current device (may be 0), any
  * contents, 16-byte aligned, not shared by calls that may run at once. out must not overlap the inputs. */
 size_t oc_b200_attention_workspace(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q);

@@ -5,7 +5,8 @@
 // key: query i of nq sees the keys j <= i + nk - nq. A row that sees no key gives zeros; a row whose
 // visible scores are all minus infinity gives NaN, as its softmax does.
 // The tables live on the device and are clamped to the tensors here, so no table value can send an
-// access out of range; a clamped value sets the device error word.
+// access out of range; a clamped value sets the device error word. A query table that decreases sets it
+// too, and no sequence of it is run: rows would have several owners, or none.
 #pragma once
 
 #include "common.cuh"
@@ -30,7 +31,10 @@ struct AttnParams {
   int* desc;            // split kernel: one descriptor per CTA
 };
 
-struct Seq { int q0, nq, k0, nk; };
+struct Seq {
+  int q0, nq, k0, nk;
+  bool down;   // the query table decreases here
+};
 
 // The first token of a sequence that sees a key (nq where none does).
 __device__ __forceinline__ int attn_first_seeing(const AttnParams& p, const Seq& s) {
@@ -52,6 +56,7 @@ __device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report 
   s.k0 = min(max(k0, 0), p.Tk);
   const int ke = min(max(k1, s.k0), p.Tk);
   s.nq = qe - s.q0;
+  s.down = q1 < q0;
   s.nk = ke - s.k0;
   bool bad = s.q0 != q0 || qe != q1 || s.k0 != k0 || ke != k1;
   if (p.kv_lens) {
@@ -63,13 +68,24 @@ __device__ __forceinline__ Seq attn_seq(const AttnParams& p, int b, bool report 
   return s;
 }
 
-// One CTA's share of the rows that no sequence owns, in front of the first one and behind the last: zeros
-// (D is a multiple of 8, rows 16-byte aligned). By `threads` threads of the CTA, of which this is `tid`.
-__device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, int cta, int n_ctas, int tid, int threads) {
+// Does the query table decrease at one of the places that this thread of `threads` looks at?
+__device__ __forceinline__ bool attn_disorder(const AttnParams& p, int tid, int threads) {
+  bool down = false;
+  if (p.cu_q)
+#pragma unroll 4
+    for (int b = tid; b < p.B; b += threads) down |= p.cu_q[b + 1] < p.cu_q[b];
+  return down;
+}
+
+// One CTA's share of the rows that no sequence owns, in front of the first one and behind the last (all of
+// them without sequences, or where `none` is run): zeros (D is a multiple of 8, rows 16-byte aligned). By
+// `threads` threads of the CTA, of which this is `tid`.
+__device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, bool none, int cta, int n_ctas, int tid,
+                                                  int threads) {
   if (!p.cu_q) return;
   const int vecs = p.D / 8;
   const int head = p.B > 0 ? min(max(p.cu_q[0], 0), p.Tq) : 0;
-  const int tail = p.B > 0 ? min(max(p.cu_q[p.B], head), p.Tq) : 0;   // without sequences every row is
+  const int tail = p.B > 0 && !none ? min(max(p.cu_q[p.B], head), p.Tq) : head;
   const long long rows = (long long)head + (p.Tq - tail);
   for (long long r = cta; r < rows; r += n_ctas) {
     const long long t = r < head ? r : tail + (r - head);

@@ -94,14 +94,19 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
   // the call's units, then this CTA's run of them (every warp finds it for itself; with up to 32
   // sequences the tables are read once)
   long long total = 0, mine = 0;
+  bool none = false;   // the table decreases: nothing is run
   for (int base = 0; base < p.B; base += 32) {
-    mine = base + lane < p.B ? split_units(p, attn_seq(p, base + lane, blockIdx.x == 0 && warp == 0)) : 0;
+    Seq x{};
+    if (base + lane < p.B) x = attn_seq(p, base + lane, blockIdx.x == 0 && warp == 0);
+    mine = base + lane < p.B ? split_units(p, x) : 0;
+    none |= __any_sync(0xffffffffu, x.down);
     long long sum = mine;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     total += sum;
   }
-  if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
+  if (none) total = 0;
+  if (p.zero_unowned) attn_zero_unowned(p, none, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
   const int busy = (int)min(total, (long long)gridDim.x);   // CTAs with work
   if ((int)blockIdx.x >= busy) return;
   long long u, u_end;

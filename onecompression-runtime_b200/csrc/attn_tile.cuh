@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += Cfg::kThreads) attn_seq(p, b, true);
   if (!work) {
-    if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
+    const bool none = __syncthreads_or(attn_disorder(p, threadIdx.x, Cfg::kThreads));
+    if (p.zero_unowned) attn_zero_unowned(p, none, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
     return;
   }
   const Seq s = w.s;
@@ -205,9 +206,17 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  const bool none = __syncthreads_or(attn_disorder(p, threadIdx.x, Cfg::kThreads));
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  if (none) {   // the table decreases: nothing is run
+    if (p.zero_unowned) attn_zero_unowned(p, true, blockIdx.x, gridDim.x, threadIdx.x, Cfg::kThreads);
+    if (tg.splits > 1 && threadIdx.x < Cfg::kRows)   // a sum of weights that no row has: the join leaves such rows alone
+      tg.part[((long long)blockIdx.x * Cfg::kTiles + threadIdx.x / 128) * (128 * (DP + 2)) + (DP + 1) * 128 +
+              threadIdx.x % 128] = -1.f;
+    if (warp == kAux + 1) tmem_dealloc(tmem, 512);
+    return;
+  }
 
   if (warp >= kAux) {
     if constexpr (kTwo) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kAuxRegs));
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::kThreads, 1)
     } else {
       // ------------------------------------------------------------ V blocks at the end of what rows see
       const int tid = threadIdx.x - (kAux + 2) * 32;
-      if (p.zero_unowned) attn_zero_unowned(p, blockIdx.x, gridDim.x, tid, 64);
+      if (p.zero_unowned) attn_zero_unowned(p, false, blockIdx.x, gridDim.x, tid, 64);
       for (int e = 0; w.e0 + e < w.nblk; ++e) {
         const int j = w.e0 + e;
         if (!mbar_wait(&edge_full[e], 0, abort_flag, kDevErrWEmpty)) break;
@@ -568,6 +577,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const AttnParams p,
   auto part = [&](int z) {
     return tg.part + (((long long)unit * tg.splits + z) * Cfg::kTiles + t) * (128 * (DP + 2)) + row;
   };
+  if (part(0)[(DP + 1) * 128] < 0.f) return;   // nothing was run
   float mx = -INFINITY;
 #pragma unroll 4
   for (int z = 0; z < tg.splits; ++z) mx = fmaxf(mx, part(z)[DP * 128]);

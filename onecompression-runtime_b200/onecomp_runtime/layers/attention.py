@@ -45,7 +45,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     together; without them all rows are one sequence). ``kv_lens``: int32 [B], how many keys from
     ``cu_seqlens_k[b]`` on are in use: a cache with room for more. They are read on the device when the kernel
     runs, so a captured graph follows their values. Values outside the tensors are clamped and set the
-    device error word (``_lib.read_device_error``).
+    device error word (``_lib.read_device_error``); a ``cu_seqlens_q`` that decreases sets it and runs no sequence
+    (a new output is all zeros, a given one stays).
 
     ``causal``: the last query of a sequence sees its last key, query i of nq the keys up to
     ``i + nk - nq``. Rows that see no key give zeros (rows whose visible scores are all minus infinity give NaN, as

@@ -139,6 +139,35 @@ def test_attention_of_an_empty_batch_with_lengths(cuda_device):
     assert e.shape == (0, 4, 64) and error_word(dev) == 0
 
 
+@pytest.mark.parametrize("heads", [(4, 2, 64), (2, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("cq", [(0, 10, 4), (0, 4, 2, 10), (7, 3), (0, 6, 4, 300), (0, 300, 299), (200, 0, 300),
+                                tuple(range(0, 280, 7)) + (0, 300), tuple(range(0, 280, 7)) + (278, 279, 5)])
+def test_attention_runs_no_sequence_of_a_decreasing_table(cuda_device, cq, heads):
+    """Rows would have several owners, or none: the table is reported, a new output is all zeros and a given one stays
+    as it was. Few rows, prompts, and keys split over CTAs; then the same call with a table in order."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    Hq, Hkv, D = heads
+    for Tk in (300, 6000):
+        q, k = randn(dev, 300, Hq, D, seed=1), randn(dev, Tk, Hkv, D, seed=2)
+        bad, ck = table(dev, *cq), table(dev, *(Tk * i // (len(cq) - 1) for i in range(len(cq))))
+        for max_q in (1, 300, None):
+            with torch.no_grad():
+                assert error_word(dev) == 0
+                dirty(dev, q)
+                o = packed_attention(q, k, k, bad, ck, max_seqlen_q=max_q)
+                assert error_word(dev) == 0x302 and bool((o == 0).all())
+                kept = torch.full_like(q, 3.0)
+                packed_attention(q, k, k, bad, ck, max_seqlen_q=max_q, out=kept)
+                assert error_word(dev) == 0x302 and bool((kept == 3).all())
+        good = table(dev, *sorted(cq))
+        seqs = [(a, b - a, c, d - c) for a, b, c, d in zip(sorted(cq), sorted(cq)[1:], ck.tolist(), ck.tolist()[1:])]
+        with torch.no_grad():
+            o = packed_attention(q, k, k, good, ck)
+        ref.check(o, *ref.attention(q, k, k, seqs, True, D ** -0.5), "table in order")
+        assert error_word(dev) == 0
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
