@@ -89,7 +89,7 @@ __device__ __forceinline__ void attn_zero_unowned(const AttnParams& p, bool none
   const long long rows = (long long)head + (p.Tq - tail);
   for (long long r = cta; r < rows; r += n_ctas) {
     const long long t = r < head ? r : tail + (r - head);
-    for (int i = tid; i < p.Hq * vecs; i += threads)
+    for (long long i = tid; i < (long long)p.Hq * vecs; i += threads)   // up to 2^35
       *reinterpret_cast<uint4*>(p.out + t * p.o_st + (i / vecs) * p.o_sh + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
   }
 }
