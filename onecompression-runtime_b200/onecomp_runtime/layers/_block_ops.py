@@ -50,9 +50,32 @@ def span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _rows_of_pitch(t: torch.Tensor) -> dict[int, int]:
+    """Ways to see the tensor as rows: {pitch: row length} in bytes, every element inside a row that begins a multiple
+    of the pitch behind the first one, and no row longer than the pitch."""
+    e = t.element_size()
+    dims = sorted((s * e, n) for n, s in zip(t.shape, t.stride()) if n > 1 and s > 0)
+    ways, length = {}, e
+    for i, (s, n) in enumerate(dims):
+        if length <= s and all(outer % s == 0 for outer, _ in dims[i + 1:]):
+            ways[s] = length
+        length += (n - 1) * s
+    ways[0] = length   # all of it as one row
+    return ways
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
-    """Whether the address ranges of two tensors meet (interleaved column slices of one buffer do)."""
+    """Whether two tensors share memory. Where their address ranges meet they do not if both are rows of one pitch that
+    lie beside one another (column slices of one buffer); tensors interleaved in other ways count as sharing."""
     if b is None:
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if not (a0 < b1 and b0 < a1):
+        return False
+    ways_a, ways_b = _rows_of_pitch(a), _rows_of_pitch(b)
+    for pitch in {*ways_a, *ways_b} - {0}:
+        la, lb = ways_a.get(pitch, ways_a[0]), ways_b.get(pitch, ways_b[0])
+        at = (b0 - a0) % pitch
+        if la <= at and at + lb <= pitch:
+            return False
+    return True

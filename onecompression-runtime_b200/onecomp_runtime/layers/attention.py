@@ -54,8 +54,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     result, not even infinities or NaN. ``scale`` defaults to ``D ** -0.5``. ``max_seqlen_q``: the longest
     query run if the host knows it; it only helps to pick the kernel (results are right whatever it says),
     and matters where one batch holds prompts beside single tokens: the mean run counts without it.
-    ``out``: [Tq, Hq, D] to write into, sharing no memory with the inputs; rows that no sequence owns stay as
-    they were (a new output holds zeros there).
+    ``out``: [Tq, Hq, D] to write into, sharing no memory with the inputs (columns of the same buffer beside
+    theirs are fine); rows that no sequence owns stay as they were (a new output holds zeros there).
     """
     what = "packed_attention"
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:

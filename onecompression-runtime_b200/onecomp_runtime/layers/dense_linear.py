@@ -51,7 +51,8 @@ def linear_fused(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     ``x`` [..., K] and ``weight`` [N, K] fp16 or bf16 of one dtype, K a multiple of 8; ``bias`` [N] fp16, bf16
     or fp32; ``activation`` None, ``"gelu_tanh"``, ``"gelu"``, ``"silu"`` or ``"relu"``; ``residual`` and
     ``out`` [..., N] in ``x``'s dtype, ``out`` may be ``residual`` itself and otherwise shares no memory with
-    the inputs. Rows of ``x`` and ``weight`` that are not contiguous or not 16-byte aligned are copied.
+    the inputs (columns of the same buffer beside theirs are fine). Rows of ``x`` and ``weight`` that are not
+    contiguous or not 16-byte aligned are copied.
     """
     what = "linear_fused"
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:

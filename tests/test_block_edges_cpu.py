@@ -1,6 +1,8 @@
 """Calls of the transformer-block operators at the edges of what their documentation allows: what the host decides."""
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
@@ -79,3 +81,51 @@ def test_attention_takes_the_lengths_of_an_empty_batch():
         packed_attention(a, a, a, none, none)
     with pytest.raises(ValueError, match="cu_seqlens_q"):
         packed_attention(a, a, a, none, one, kv_lens=none)
+
+
+def addresses(t):
+    """The byte addresses of a tensor's elements."""
+    if t.numel() == 0:
+        return set()
+    at = torch.zeros(t.shape, dtype=torch.int64)
+    for d, (n, s) in enumerate(zip(t.shape, t.stride())):
+        at += (torch.arange(n) * s).view([-1 if i == d else 1 for i in range(t.dim())])
+    e = t.element_size()
+    return {t.data_ptr() + e * int(x) + i for x in at.flatten() for i in range(e)}
+
+
+def test_shared_memory_is_seen():
+    """Random strided tensors over one buffer: whatever shares a byte is found to share memory."""
+    from onecomp_runtime.layers._block_ops import overlap
+    rng, found = random.Random(3), [0, 0]
+    buf = torch.zeros(4096, dtype=torch.int16)
+    for _ in range(3000):
+        pair = []
+        for _ in range(2):
+            n = rng.choice([1, 2, 3])
+            shape = [rng.choice([1, 2, 3, 5]) for _ in range(n)]
+            stride = [rng.choice([0, 1, 2, 4, 6, 8, 16, 24, 48, 96]) for _ in range(n)]
+            x = buf.as_strided(shape, stride, rng.randrange(200))
+            pair.append(x if rng.random() < 0.8 or any(s % 2 for s in stride) else
+                        buf.view(torch.float32).as_strided(shape, [s // 2 for s in stride], rng.randrange(100)))
+        a, b = pair
+        shares = bool(addresses(a) & addresses(b))
+        assert overlap(a, b) == overlap(b, a)
+        assert overlap(a, b) or not shares, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        found[shares] += 1
+    assert min(found) > 300
+
+
+def test_slices_of_one_buffer_share_nothing():
+    """What a user keeps side by side in one buffer: columns of a projection, a head's parts, blocks of rows."""
+    from onecomp_runtime.layers._block_ops import overlap
+    b = zeros(7, 6 * 64)
+    q, o = b[:, :128].unflatten(1, (2, 64)), b[:, 256:].unflatten(1, (2, 64))
+    heads = zeros(7, 4, 3, 64)
+    batch = zeros(2, 5, 96)
+    for x, y in ((q, o), (b[:, :100], b[:, 100:]), (heads[:, :, 0], heads[:, :, 2]), (batch[..., :32], batch[..., 32:]),
+                 (b[:3], b[3:]), (b[:, :64], b[2, 64:]), (b[1:, :8], b[:-1, 376:]), (heads[:, 0], heads[:, 1:]),
+                 (heads[:, :, 1, :8], heads[:, :, 1, 8:])):
+        assert not overlap(x, y) and not overlap(y, x) and not addresses(x) & addresses(y)
+    for x, y in ((q, b[:, 64:192].unflatten(1, (2, 64))), (b[:, :101], b[:, 100:]), (b[:4], b[3:]), (b, b), (b[:, 64:], b[2, 64:])):
+        assert overlap(x, y) and overlap(y, x)

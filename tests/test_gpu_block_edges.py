@@ -168,6 +168,24 @@ def test_attention_runs_no_sequence_of_a_decreasing_table(cuda_device, cq, heads
         assert error_word(dev) == 0
 
 
+@pytest.mark.parametrize("T", [3, 300])
+def test_attention_writes_beside_its_inputs(cuda_device, T):
+    """q, k, v and the output as columns of one buffer share no memory: the result is that of separate tensors and
+    nothing else in the buffer changes. Columns that do meet are refused."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    buf = randn(dev, T, 10 * 64, seed=1)
+    q, k, v, out, rest = (buf[:, a * 64:b * 64].unflatten(1, (-1, 64)) for a, b in ((0, 2), (2, 4), (4, 6), (6, 8), (8, 10)))
+    before = buf.clone()
+    with torch.no_grad():
+        want = packed_attention(q.contiguous(), k.contiguous(), v.contiguous())
+        got = packed_attention(q, k, v, out=out)
+        assert torch.equal(got, want) and torch.equal(buf[:, :384], before[:, :384]) and torch.equal(rest, before[:, 512:].view_as(rest))
+        for bad in (q, buf[:, 64:192].unflatten(1, (2, 64)), buf[:, 320:448].unflatten(1, (2, 64))):
+            with pytest.raises(ValueError, match="shares memory"):
+                packed_attention(q, k, v, out=bad)
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
@@ -193,3 +211,26 @@ def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
     mag = mag * far.unsqueeze(1)
     tol = tol + torch.cat([mag, mag], -1)
     ref.check(y, want, tol, "far positions")
+
+
+# ---------------------------------------------------------------------------------------- dense linear
+@pytest.mark.parametrize("M", [5, 60, 300])
+def test_linear_writes_beside_its_inputs(cuda_device, M):
+    """x, the residual and the output as columns of one buffer, on 16-byte boundaries and off them."""
+    from onecomp_runtime.layers import linear_fused
+    dev = cuda_device
+    K, N = 128, 200
+    for shift in (0, 3):
+        buf = randn(dev, M, K + 3 * N, seed=M)
+        w = randn(dev, N, K, seed=2, std=K ** -0.5)
+        x, r, out = buf[:, :K], buf[:, K + shift:K + N + shift], buf[:, K + N + shift:K + 2 * N + shift]
+        before = buf.clone()
+        with torch.no_grad():
+            got = linear_fused(x, w, residual=r, out=out)
+            ref.check(got, *ref.linear(before[:, :K], w, None, None, before[:, K + shift:K + N + shift]), "beside")
+            assert torch.equal(buf[:, :K + N + shift], before[:, :K + N + shift])
+            assert torch.equal(buf[:, K + 2 * N + shift:], before[:, K + 2 * N + shift:])
+            for bad in (buf[:, K - 1:K - 1 + N], buf[:, K + shift + 1:K + shift + 1 + N]):
+                with pytest.raises(ValueError):
+                    linear_fused(x, w, residual=r, out=bad)
+    assert error_word(dev) == 0
