@@ -43,9 +43,7 @@ def on_device(dev: torch.device):
 
 
 def span(t: torch.Tensor) -> tuple[int, int]:
-    """First byte and one past the last byte that the tensor's elements touch."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
+    """First byte and one past the last byte that the elements of a tensor, of one at least, touch."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
@@ -67,7 +65,7 @@ def _rows_of_pitch(t: torch.Tensor) -> dict[int, int]:
 def overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
     """Whether two tensors share memory. Where their address ranges meet they do not if both are rows of one pitch that
     lie beside one another (column slices of one buffer); tensors interleaved in other ways count as sharing."""
-    if b is None:
+    if b is None or a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
     if not (a0 < b1 and b0 < a1):

@@ -7,7 +7,7 @@ import math
 import torch
 
 from .. import _lib
-from ._block_ops import MAX_COUNT, inference_only, on_device, one_device
+from ._block_ops import MAX_COUNT, inference_only, on_device, one_device, overlap
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None
@@ -91,6 +91,16 @@ def _in_place(what: str, t: torch.Tensor, T: int) -> tuple:
         if (n0 > 1 and s0 < D) or (n1 > 1 and s1 < (max(s0 * (n0 - 1) + D, D) if n0 > 1 else D)):
             raise ValueError(f"{what}: in place on overlapping rows (strides {t.stride()})")
     return x.data_ptr(), st, sh, x.data_ptr(), st, sh, H
+
+
+def _may_overlap(a: tuple, b: tuple, D: int, size: int) -> bool:
+    """False for the kernel arguments of two slices beside one another in one projection's output, the common case,
+    without walking their dimensions (:func:`overlap` does for the others)."""
+    pitch = a[1]
+    if pitch != b[1] or pitch <= 0:
+        return True
+    at = (b[0] - a[0]) // size % pitch
+    return at < (a[6] - 1) * a[2] + D or at + (b[6] - 1) * b[2] + D > pitch
 
 
 class RotaryEmbedding(torch.nn.Module):
@@ -191,10 +201,10 @@ class RotaryEmbedding(torch.nn.Module):
         dev = one_device(what, q, k, positions)
         if inplace:
             q_out, k_out = q, k
-            if k is not None and k.data_ptr() == q.data_ptr() and q.numel() and k.numel():
-                raise ValueError(f"{what}: in place on q and k that begin at one address")
             q_args = _in_place(what, q, T)
             k_args = _NO_TENSOR if k is None else _in_place(what, k, T)
+            if k is not None and _may_overlap(q_args, k_args, D, q.element_size()) and overlap(q, k):
+                raise ValueError(f"{what}: in place on q and k that share memory")
         else:
             q, q_out, q_args = _out_of_place(q, T, D, dtype, dev)
             k_out, k_args = None, _NO_TENSOR

@@ -129,3 +129,33 @@ def test_slices_of_one_buffer_share_nothing():
         assert not overlap(x, y) and not overlap(y, x) and not addresses(x) & addresses(y)
     for x, y in ((q, b[:, 64:192].unflatten(1, (2, 64))), (b[:, :101], b[:, 100:]), (b[:4], b[3:]), (b, b), (b[:, 64:], b[2, 64:])):
         assert overlap(x, y) and overlap(y, x)
+
+
+def test_rotary_in_place_refuses_shared_memory(monkeypatch):
+    """q and k that meet anywhere would be rotated twice or half; slices beside one another go on (here to the device's
+    refusal, which comes first, so it is taken out of the way and the launch with it)."""
+    from onecomp_runtime.layers import RotaryEmbedding, rotary
+    rope, pos, launched = RotaryEmbedding(64), torch.arange(6), []
+    monkeypatch.setattr(rotary, "one_device", lambda what, q, *more: q.device)
+    monkeypatch.setattr(rotary.RotaryEmbedding, "_table", lambda self, dev: (pos, None))
+    monkeypatch.setattr(rotary, "on_device", lambda dev: torch.no_grad())
+    monkeypatch.setattr(rotary._lib, "stream_of", lambda dev: 0)
+    monkeypatch.setattr(rotary._lib, "call", lambda *a: launched.append(a))
+    b = zeros(6, 8 * 64)
+
+    def heads(lo, hi):
+        return b[:, lo * 64:hi * 64].unflatten(1, (hi - lo, 64))
+
+    inner = zeros(6, 4, 3, 64)
+    for q, k in ((heads(0, 4), heads(4, 6)), (heads(4, 8), heads(0, 4)), (b[:3].view(3, 8, 64), b[3:].view(3, 8, 64)),
+                 (inner[:, :, 0], inner[:, :, 1]), (zeros(6, 2, 64), zeros(6, 2, 64)), (heads(0, 2)[:1], heads(1, 3)[1:2])):
+        rope(q, k, pos[:len(q)], inplace=True)
+    assert len(launched) == 6
+    rope(heads(0, 4), heads(2, 2), pos, inplace=True)      # no key head: nothing to share
+    launched.pop()
+    for q, k in ((heads(0, 4), heads(0, 4)), (heads(0, 4), heads(3, 6)), (heads(2, 4), heads(1, 3)), (heads(3, 4), heads(0, 8)),
+                 (b[:4].view(4, 8, 64), b[2:].view(4, 8, 64)), (inner[:, :, 0], inner[:, 0]),
+                 (b[:, 1:129].unflatten(1, (2, 64)), heads(2, 3))):
+        with pytest.raises(ValueError, match="share memory"):
+            rope(q, k, pos[:len(q)], inplace=True)
+    assert len(launched) == 6
