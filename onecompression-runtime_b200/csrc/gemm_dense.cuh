@@ -184,15 +184,17 @@ __global__ void __launch_bounds__(kDsThreads)
       uint16_t* dst = p.out + m * p.ldc + n;
       const uint16_t* res = p.residual ? p.residual + m * p.ldr + n : nullptr;
       const int nf = min(8, p.N - n);
-      uint16_t rv[8];
+      alignas(16) uint16_t rv[8];   // moved as one 16-byte vector where the rows allow
       if (res) {
         if (p.vec && nf == 8) {
           *reinterpret_cast<uint4*>(rv) = *reinterpret_cast<const uint4*>(res);
         } else {
-          for (int e = 0; e < nf; ++e) rv[e] = res[e];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < nf) rv[e] = res[e];
         }
       }
-      uint16_t ov[8];
+      alignas(16) uint16_t ov[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (e < nf) {
@@ -205,7 +207,9 @@ __global__ void __launch_bounds__(kDsThreads)
       if (p.vec && nf == 8) {
         *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(ov);
       } else {
-        for (int e = 0; e < nf; ++e) dst[e] = ov[e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < nf) dst[e] = ov[e];
       }
     }
   }
