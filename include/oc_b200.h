@@ -337,6 +337,9 @@ int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
 int oc_b200_dense_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int M, int N, int K,
                        const void* bias, int bias_dtype, const void* residual, int64_t ldr, int act, void* c,
                        int64_t ldc, oc_stream_t stream);
+/* The tokens of the tiles that such a call of these sizes works in on the current device, and whether its kernel
+ * splits K over a cluster (few tokens) or walks it in CTA pairs. */
+int oc_b200_dense_gemm_tile(int M, int N, int K, int* tokens, int* splits_k);
 
 #ifdef __cplusplus
 }

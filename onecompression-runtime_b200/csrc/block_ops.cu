@@ -220,6 +220,19 @@ int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, o
   return launch_check("dense_gemm");
 }
 
+// Tokens of a tile of the K-splitting kernel, or 0 where the pairs take the call.
+// The K-splitting kernel up to 32 tokens, where streaming the weights through every SM decides (one token,
+// weights from HBM, 4096 x 4096: 12.8 us against 16.8 of the pairs; 1024 x 8192: 10.8 against 27.1). Above, the
+// pairs (64 tokens, 2560 x 2560: 13.9 against 11.8), unless few of them would walk a long K (64 tokens,
+// 1024 x 8192: 13.8 against 26.9; 128 tokens: 16.2 against 25.1).
+int dense_split_tokens(int M, int N, int K) {
+  const int least_tiles = (N + 255) / 256 * ((M + 31) / 32);   // of the pairs, at 32 tokens each
+  if (M <= 16) return 16;
+  if (M <= 32) return 32;
+  if (M <= 128 && least_tiles <= 24 && K > 4096) return M <= 64 ? 64 : 128;
+  return 0;
+}
+
 // Tokens of a tile for the pair kernel: equal tiles of a multiple of 32 tokens, the size with the least
 // (waves of CTA pairs) x (time of one tile). A 64-k step of a tile takes about 2.3 cycles per token
 // (measured 590 at 256 tokens, 295 at 128), but no less than about 250, where the weights' stream bounds
@@ -229,7 +242,7 @@ int dense_bt(int M, int tiles_n, int K, int pairs) {
   const int kb = (K + 63) / 64;
   int best = 256;
   double best_cost = 1e300;
-  for (int want = 256; want >= 32; want -= 32) {
+  for (int want = 256; want >= 64; want -= 32) {   // below 64 a tile takes no less time
     const int tiles_m = (M + want - 1) / want;
     const int bt = ((M + tiles_m - 1) / tiles_m + 31) / 32 * 32;
     const double waves = std::ceil((double)tiles_n * tiles_m / pairs);
@@ -300,16 +313,11 @@ int launch_dense_tile_act(const void* x, int64_t ldx, const void* w, int64_t ldw
 template <bool BF16>
 int launch_dense(const void* x, int64_t ldx, const void* w, int64_t ldw, const oc::DenseParams& p, int dev,
                  cudaStream_t stream) {
-  // The K-splitting kernel up to 32 tokens, where streaming the weights through every SM decides (one token,
-  // weights from HBM, 4096 x 4096: 12.8 us against 16.8 of the pairs; 1024 x 8192: 10.8 against 27.1). Above, the
-  // pairs (64 tokens, 2560 x 2560: 13.9 against 11.8), unless few of them would walk a long K (64 tokens,
-  // 1024 x 8192: 13.8 against 26.9; 128 tokens: 16.2 against 25.1).
-  const int least_tiles = (p.N + 255) / 256 * ((p.M + 31) / 32);   // of the pairs, at their smallest size
-  if (p.M <= 16) return launch_dense_split<BF16, 16>(x, ldx, w, ldw, p, dev, stream);
-  if (p.M <= 32) return launch_dense_split<BF16, 32>(x, ldx, w, ldw, p, dev, stream);
-  if (p.M <= 128 && least_tiles <= 24 && p.K > 4096)
-    return p.M <= 64 ? launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream)
-                     : launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
+  const int split = dense_split_tokens(p.M, p.N, p.K);
+  if (split == 16) return launch_dense_split<BF16, 16>(x, ldx, w, ldw, p, dev, stream);
+  if (split == 32) return launch_dense_split<BF16, 32>(x, ldx, w, ldw, p, dev, stream);
+  if (split == 64) return launch_dense_split<BF16, 64>(x, ldx, w, ldw, p, dev, stream);
+  if (split == 128) return launch_dense_split<BF16, 128>(x, ldx, w, ldw, p, dev, stream);
   return p.residual ? launch_dense_tile_act<BF16, true>(x, ldx, w, ldw, p, dev, stream)
                     : launch_dense_tile_act<BF16, false>(x, ldx, w, ldw, p, dev, stream);
 }
@@ -425,6 +433,18 @@ extern "C" int oc_b200_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   if (dp == 64) return bf16 ? launch_split<true, 64>(p, ctas, stream) : launch_split<false, 64>(p, ctas, stream);
   if (dp == 128) return bf16 ? launch_split<true, 128>(p, ctas, stream) : launch_split<false, 128>(p, ctas, stream);
   return bf16 ? launch_split<true, 256>(p, ctas, stream) : launch_split<false, 256>(p, ctas, stream);
+}
+
+extern "C" int oc_b200_dense_gemm_tile(int M, int N, int K, int* tokens, int* splits_k) {
+  if (!tokens || !splits_k) return fail(OC_ERR_INVALID, "dense_gemm_tile: NULL pointer");
+  if (M <= 0 || N <= 0 || K <= 0 || too_many(M) || too_many(N) || too_many(K))
+    return fail(OC_ERR_INVALID, "dense_gemm_tile: M=%d N=%d K=%d (above 0, below 2^30)", M, N, K);
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  *tokens = dense_split_tokens(M, N, K);
+  *splits_k = *tokens != 0;
+  if (!*tokens) *tokens = dense_bt(M, (N + 255) / 256, K, sm_count(dev) / 2);
+  return OC_OK;
 }
 
 extern "C" int oc_b200_dense_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int M, int N,

@@ -84,6 +84,7 @@ _SIGNATURES = {
     "oc_b200_attention": ([_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _i, _i, _p,
                            _p, _p, _i, _i, ctypes.c_float, _i, _i, _p, _sz, _p], _i),
     "oc_b200_dense_gemm": ([_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i, _p, _i64, _i, _p, _i64, _p], _i),
+    "oc_b200_dense_gemm_tile": ([_i, _i, _i, _p, _p], _i),
 }
 
 

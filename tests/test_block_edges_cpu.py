@@ -159,3 +159,13 @@ def test_rotary_in_place_refuses_shared_memory(monkeypatch):
         with pytest.raises(ValueError, match="share memory"):
             rope(q, k, pos[:len(q)], inplace=True)
     assert len(launched) == 6
+
+
+def test_dense_tile_query_refuses():
+    import ctypes
+    from onecomp_runtime import _lib
+    lib, n, f = _lib.lib(), ctypes.c_int(), ctypes.c_int()
+    for args in ((0, 8, 8), (8, 0, 8), (8, 8, -8), (1 << 30, 8, 8), (8, 1 << 30, 8), (8, 8, 1 << 30)):
+        assert lib.oc_b200_dense_gemm_tile(*args, ctypes.byref(n), ctypes.byref(f)) == 1
+    assert lib.oc_b200_dense_gemm_tile(8, 8, 8, None, ctypes.byref(f)) == 1
+    assert lib.oc_b200_dense_gemm_tile(8, 8, 8, ctypes.byref(n), None) == 1

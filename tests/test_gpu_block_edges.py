@@ -234,3 +234,59 @@ def test_linear_writes_beside_its_inputs(cuda_device, M):
                 with pytest.raises(ValueError):
                     linear_fused(x, w, residual=r, out=bad)
     assert error_word(dev) == 0
+
+
+def dense_tile(M, N, K):
+    import ctypes
+    from onecomp_runtime import _lib
+    tokens, splits = ctypes.c_int(), ctypes.c_int()
+    _lib.call("oc_b200_dense_gemm_tile", M, N, K, ctypes.byref(tokens), ctypes.byref(splits))
+    return tokens.value, bool(splits.value)
+
+
+def test_linear_tile_rule(cuda_device):
+    """Few tokens split K; the pairs' tiles are multiples of 32 tokens, no longer than the call needs."""
+    for M in (1, 16, 17, 32, 33, 64, 65, 128, 129, 300, 517, 1024, 4099):
+        for N, K in ((8, 8), (2560, 2560), (1024, 8192), (8200, 5120), (95000, 64)):
+            tokens, splits = dense_tile(M, N, K)
+            assert splits or (64 <= tokens <= 256 and tokens % 32 == 0)
+            assert splits or -(-M // tokens) * tokens - M < 32 * -(-M // tokens)
+            assert splits == (M <= 32 or (M <= 128 and K > 4096 and -(-N // 256) * -(-M // 32) <= 24))
+
+
+PAIR_TILES = [   # M, N, K, tokens of a tile: at least 5 tiles for each of 74 pairs, ragged in both dimensions
+    (57, 94984, 72, 64), (91, 95001, 136, 96), (113, 94984, 200, 128), (155, 95001, 72, 160), (187, 94984, 72, 192),
+    (211, 95001, 72, 224), (251, 94984, 72, 256), (449, 40008, 1032, 160), (513, 31992, 72, 192), (577, 31997, 136, 224),
+    (673, 31992, 264, 256), (1300, 20104, 520, 224), (4099, 6344, 1032, 256)]
+
+
+@pytest.mark.parametrize("case", PAIR_TILES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_linear_many_tiles_for_each_pair(cuda_device, case, dtype):
+    """Every tile size over many tiles: both accumulators and every buffer are used again and again, bands of feature
+    tiles end early, and both epilogues write, with a residual, the residual as the output, and without one."""
+    from onecomp_runtime.layers import linear_fused
+    dev = cuda_device
+    M, N, K, tokens = case
+    assert dense_tile(M, N, K) == (tokens, False)
+    tiles_n = -(-N // 256)
+    assert tiles_n * -(-M // tokens) >= 5 * 74 and tiles_n > 8 and tiles_n % 8 and M % tokens and N % 256
+    x, w, b = randn(dev, M, K, dtype=dtype, seed=1), randn(dev, N, K, dtype=dtype, seed=2, std=K ** -0.5), \
+        randn(dev, N, dtype=torch.float32, seed=3)
+    r = randn(dev, M, N, dtype=dtype, seed=4)
+    with torch.no_grad():
+        want, tol = ref.linear(x, w, b, "gelu_tanh", None)
+        first = linear_fused(x, w, b, activation="gelu_tanh")
+        ref.check(first, want, tol, f"{case}")
+        assert all(torch.equal(first, linear_fused(x, w, b, activation="gelu_tanh")) for _ in range(3))
+        del want, tol, first
+        want, tol = ref.linear(x, w, b, "relu", r)
+        ref.check(linear_fused(x, w, b, activation="relu", residual=r), want, tol, f"{case} residual")
+        acc = r.clone()
+        ref.check(linear_fused(x, w, b, activation="relu", residual=acc, out=acc), want, tol, f"{case} onto the residual")
+        wide = torch.full((M, N + 3), 7.0, dtype=dtype, device=dev)    # rows off 16-byte boundaries
+        wide[:, 1:N + 1] = r
+        at = wide[:, 1:N + 1]
+        ref.check(linear_fused(x, w, b, activation="relu", residual=at, out=at), want, tol, f"{case} direct stores")
+        assert bool((wide[:, 0] == 7).all()) and bool((wide[:, N + 1:] == 7).all())
+    assert error_word(dev) == 0
