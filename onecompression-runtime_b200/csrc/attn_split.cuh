@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::kThreads, SplitCfg<DP>::kCtasPer
         for (int t = 0; t < 2; ++t) {
           const float p0 = ex2(c[t][2 * i] - ref), p1 = ex2(c[t][2 * i + 1] - ref);
           l[i] += p0 + p1;
-          pa[2 * t + i] = pack2_rn<BF16>(p0, p1);   // the weights as the product's 16-bit operand
+          pa[2 * t + i] = pack2_rn<BF16>(p0, p1);   // rounded once, as the product takes them; l adds them unrounded
         }
       }
       // A value that a row does not see may be infinite or NaN, and its weight of zero must not turn that

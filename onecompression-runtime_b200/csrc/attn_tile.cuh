@@ -1,14 +1,16 @@
 // Attention for prompts: many query rows per sequence, on the 5th-generation tensor cores.
 //
 // Bound by the tensor pipe and, at head size 64 and 128, by the exponentials (16 a cycle and SM against
-// 8192 tensor operations). One CTA per 128-row tile pair of one query head (one tile where the head
-// size is 256): S = Q K^T and O += P V as tcgen05 MMAs of 128 x 128 x 16 into TMEM, one pass over the
-// keys in blocks of 128.
+// 8192 tensor operations). The (token, head) rows of a key head's query heads are packed into tiles of
+// 128 rows, two tiles to a CTA (one where the head size is 256): S = Q K^T and O += P V as tcgen05 MMAs of
+// 128 x 128 x 16 into TMEM, one pass over the keys in blocks of 128.
 //   * A softmax warpgroup per tile, one thread per row: it reads S from TMEM (no shuffles), writes the
-//     16-bit weights P back to TMEM as the A operand of the second product, and keeps maximum and sum
-//     in registers. Each tile's products are issued by a thread of their own: while one tile is in its
-//     softmax the tensor pipe runs the other's, and the second product starts on the first 96 keys'
-//     weights while the softmax works on the rest.
+//     weights P back to TMEM as the A operand of the second product, and keeps maximum and sum in registers.
+//     P is rounded to 16 bits once, as the product takes it (half a step of each weight; the sum adds
+//     the unrounded ones, so the error does not grow with the keys).
+//   * One warp issues both tiles' products in turn: while one tile is in its softmax the tensor pipe runs
+//     the other's, and the second product starts on the first 96 keys' weights while the softmax works
+//     on the rest.
 //   * The reference that the exponents are taken against follows the running maximum only when
 //     it grows by more than 2^8: weights up to 256 are as exact in 16 bits as weights up to 1, and
 //     the accumulator in TMEM is read, scaled and written back only in those rare steps.

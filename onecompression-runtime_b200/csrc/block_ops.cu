@@ -182,6 +182,7 @@ template <bool BF16, int DP> int launch_tile(oc::AttnParams p, const oc::TileGri
   kern<<<(unsigned)(units * tg.splits), Cfg::kThreads, Cfg::kSmem, stream>>>(maps, p, tg, mode);
   if (int rc = launch_check("attention (tile)")) return rc;
   if (tg.splits == 1) return OC_OK;
+  // the tile kernel gives no signal, yet this launch starts 0.7 us earlier than a plain one (7 x 5 tokens, heads of 256)
   return launch_pdl(oc::attn_tile_join_kernel<BF16, DP>, dim3((unsigned)(units * Cfg::kTiles), 4, DP / 64), dim3(256), 0, stream,
                     "attention (tile join)", p, tg);
 }

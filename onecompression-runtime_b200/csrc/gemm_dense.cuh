@@ -8,7 +8,8 @@ namespace oc {
 
 // Epilogue activations of the dense linear (the first two are Act's). Each is evaluated so that its
 // relative error stays near fp32's where the value is small: tanh-GELU as v / (1 + e^-2u) instead of
-// a difference of numbers close to 1, GELU through the normal distribution function.
+// a difference of numbers close to 1, GELU through the normal distribution function. The fast exponential
+// and division are off by 2^-16 at most, and by less where results are not tiny: below half a step (2^-11, 2^-8).
 enum DenseAct : int { kDenseNone = 0, kDenseGeluTanh = 1, kDenseGelu = 2, kDenseSilu = 3, kDenseRelu = 4 };
 
 __device__ __forceinline__ float dense_act(float v, int act) {
