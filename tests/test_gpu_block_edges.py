@@ -290,3 +290,34 @@ def test_linear_many_tiles_for_each_pair(cuda_device, case, dtype):
         ref.check(linear_fused(x, w, b, activation="relu", residual=at, out=at), want, tol, f"{case} direct stores")
         assert bool((wide[:, 0] == 7).all()) and bool((wide[:, N + 1:] == 7).all())
     assert error_word(dev) == 0
+
+
+@pytest.mark.parametrize("act", [None, "gelu_tanh", "gelu", "silu", "relu"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M", [24, 290])
+def test_linear_activations_of_extreme_values(cuda_device, act, dtype, M):
+    """Sums that are huge, tiny, infinite or NaN come out of every activation as its formula has them."""
+    from onecomp_runtime.layers import linear_fused
+    dev = cuda_device
+    top = torch.finfo(dtype).max
+    vals = [0.0, 1e-7, -1e-7, 0.5, -0.5, 5.0, -5.0, 12.0, -12.0, 44.0, -44.0, 100.0, -100.0, 6e4, -6e4, top, -top, math.inf,
+            -math.inf, math.nan]
+    x = torch.zeros(M, 16, dtype=dtype, device=dev)
+    x[:, 0] = torch.tensor(vals, dtype=torch.float64, device=dev).to(dtype).repeat(-(-M // len(vals)))[:M]
+    w = torch.zeros(264, 16, dtype=dtype, device=dev)
+    w[:, 0] = 1
+    with torch.no_grad():
+        y = linear_fused(x, w, activation=act)
+    v = x[:, :1].double().expand(M, 264)
+    # (the normal distribution function through erfc: 1 + erf loses it below -6, where it is 1e-9 and less)
+    want = 0.5 * v * torch.special.erfc(-v / math.sqrt(2.0)) if act == "gelu" else ref.act64(v, act)
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    ok = ~torch.isnan(want)
+    exact = want.to(dtype).double()      # infinities and what rounds to them
+    inf = ok & torch.isinf(exact)
+    assert torch.equal(y[inf].double(), exact[inf])
+    fin = ok & ~inf
+    # the exponent of the fast exponential is off by 2^-16 of the result at most; below the type's normal range one step
+    tol = want.abs() * (ref.half_step(dtype) + 2.0 ** -16) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    ref.check(y[fin], want[fin], tol[fin], f"{act}")
+    assert error_word(dev) == 0
