@@ -306,7 +306,7 @@ int oc_b200_nvls_allreduce_rmsnorm_bf16(void* mc_ptr, int rows, int cols, const 
  * position * turns[i] / 2^64 of a full turn and is multiplied by gain. positions: int32 or int64
  * [T, axes], rows positions_st elements apart; axis[i] picks pair i's column (NULL: column 0, and
  * every axis[i] must be a column). turns, axis: device arrays of R/2. q_out / k_out may be the inputs;
- * out of place the D - R values behind the rotated part are copied. */
+ * out of place the D - R values behind the rotated part are copied, and D is even. */
 int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int Hq,
                  const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int Hk,
                  int dtype, int T, int D, int R, const void* positions, int positions_64, int64_t positions_st,

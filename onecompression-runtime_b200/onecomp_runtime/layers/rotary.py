@@ -106,7 +106,8 @@ def _may_overlap(a: tuple, b: tuple, D: int, size: int) -> bool:
 class RotaryEmbedding(torch.nn.Module):
     """Rotates queries and keys by their positions (``oc_b200_rope``, one launch for both).
 
-    ``rotary_dim`` of the ``head_dim`` values are rotated (default all; the rest passes through). ``layout``:
+    ``rotary_dim`` of the ``head_dim`` values are rotated (default all; the rest passes through, and is copied in pairs:
+    an odd head size works in place only). ``layout``:
     ``"half"`` pairs value i with i + rotary_dim/2, ``"interleaved"`` pairs neighbours. ``axes``: sizes that
     sum to ``rotary_dim`` for tokens with several coordinates (time, height, width); the pairs of section a
     turn by coordinate a, with the frequencies of a head of that size. ``scaling``: see
@@ -197,6 +198,8 @@ class RotaryEmbedding(torch.nn.Module):
         T = q_shape[0] if len(tokens) == 1 else math.prod(tokens)
         if max(T, q_shape[-2], 0 if k is None else k.shape[-2]) > MAX_COUNT:
             raise ValueError(f"{what}: {T} tokens, {q_shape[-2]} query heads (each below 2**30)")
+        if D % 2 and not inplace:
+            raise ValueError(f"{what}: head size {D} must be even out of place")
         inference_only(what, q, k)
         dev = one_device(what, q, k, positions)
         if inplace:

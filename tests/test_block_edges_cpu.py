@@ -169,3 +169,19 @@ def test_dense_tile_query_refuses():
         assert lib.oc_b200_dense_gemm_tile(*args, ctypes.byref(n), ctypes.byref(f)) == 1
     assert lib.oc_b200_dense_gemm_tile(8, 8, 8, None, ctypes.byref(f)) == 1
     assert lib.oc_b200_dense_gemm_tile(8, 8, 8, ctypes.byref(n), None) == 1
+
+
+def test_rotary_odd_heads_out_of_place_are_refused():
+    """The values behind the rotated part are copied in pairs; in place nothing is copied (and the CPU is refused)."""
+    import ctypes
+    from onecomp_runtime import _lib
+    from onecomp_runtime.layers import RotaryEmbedding
+    rope, x = RotaryEmbedding(65, rotary_dim=64), zeros(3, 2, 65)
+    with pytest.raises(ValueError, match="even out of place"):
+        rope(x, None, torch.arange(3))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rope(x, None, torch.arange(3), inplace=True)
+    p, o = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x20000)
+    assert _lib.lib().oc_b200_rope(p, 130, 65, o, 130, 65, 2, None, 0, 0, None, 0, 0, 0, 1, 3, 65, 64, p, 1, 1, p, None, 1.0, 0,
+                                   None) == 1
+    assert "even out of place" in _lib.last_error()

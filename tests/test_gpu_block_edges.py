@@ -213,6 +213,18 @@ def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
     ref.check(y, want, tol, "far positions")
 
 
+def test_rope_odd_head_size_in_place(cuda_device):
+    from onecomp_runtime.layers import RotaryEmbedding
+    dev = cuda_device
+    for layout in ("half", "interleaved"):
+        rope, pos = RotaryEmbedding(65, rotary_dim=62, layout=layout), torch.arange(9, device=dev)
+        q = randn(dev, 9, 3, 65, seed=2)
+        want = ref.rope(q, pos.double()[:, None] * torch.tensor(rope.inv_freq, dtype=torch.float64, device=dev), 1.0, 62,
+                        layout == "interleaved")
+        with torch.no_grad():
+            ref.check(rope(q, None, pos, inplace=True)[0], *want, layout)
+
+
 # ---------------------------------------------------------------------------------------- dense linear
 @pytest.mark.parametrize("M", [5, 60, 300])
 def test_linear_writes_beside_its_inputs(cuda_device, M):
