@@ -60,7 +60,7 @@ bool too_many(int n) { return n >= 1 << 30; }
 template <int DT, int V, bool INTER>
 int launch_rope(const oc::RopeParams& p0, int sms, cudaStream_t stream) {
   oc::RopeParams p = p0;
-  const int heads = p.t[0].H + p.t[1].H;
+  const long long heads = (long long)p.t[0].H + p.t[1].H;
   // Four tokens to a block once that still gives every SM several blocks; below, one token, its heads
   // spread over blocks until about two blocks per SM run.
   const int tb = p.T >= 4 * 4 * sms ? 4 : 1;
@@ -333,8 +333,8 @@ extern "C" int oc_b200_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_o
   if (T < 0 || Hq < 0 || Hk < 0 || D <= 0 || D > 1024 || R <= 0 || R > D || R % 2 != 0)
     return fail(OC_ERR_INVALID, "rope: T=%d Hq=%d Hk=%d D=%d R=%d (R even, at most D; D at most 1024)", T, Hq, Hk, D, R);
   if (!dtf(dtype)) return fail(OC_ERR_INVALID, "rope: dtype %d", dtype);
-  if (Hq > 65535 || Hk > 65535) return fail(OC_ERR_INVALID, "rope: %d + %d heads", Hq, Hk);
-  if (too_many(T)) return fail(OC_ERR_INVALID, "rope: %d tokens", T);
+  if (too_many(T) || too_many(Hq) || too_many(Hk))
+    return fail(OC_ERR_INVALID, "rope: T=%d Hq=%d Hk=%d (below 2^30)", T, Hq, Hk);
   if (T == 0 || Hq + Hk == 0) return OC_OK;
   if ((Hq && (!q || !q_out)) || (Hk && (!k || !k_out)) || !positions || !turns)
     return fail(OC_ERR_INVALID, "rope: NULL pointer");

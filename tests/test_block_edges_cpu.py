@@ -185,3 +185,17 @@ def test_rotary_odd_heads_out_of_place_are_refused():
     assert _lib.lib().oc_b200_rope(p, 130, 65, o, 130, 65, 2, None, 0, 0, None, 0, 0, 0, 1, 3, 65, 64, p, 1, 1, p, None, 1.0, 0,
                                    None) == 1
     assert "even out of place" in _lib.last_error()
+
+
+def test_rotary_counts_of_heads():
+    """Heads up to 2^30, as the header says; more are refused before any launch."""
+    import ctypes
+    from onecomp_runtime import _lib
+    from onecomp_runtime.layers import RotaryEmbedding
+    p = ctypes.c_void_p(0x10000)
+    for Hq, Hk in ((1 << 30, 0), (1, 1 << 30)):
+        assert _lib.lib().oc_b200_rope(p, 8, 8, p, 8, 8, Hq, p, 8, 8, p, 8, 8, Hk, 1, 1, 8, 8, p, 1, 1, p, None, 1.0, 0, None) == 1
+        assert "below 2^30" in _lib.last_error()
+    one = zeros(1, 1, 8)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        RotaryEmbedding(8)(one, one.expand(1, 2**30, 8), torch.arange(1))

@@ -225,6 +225,19 @@ def test_rope_odd_head_size_in_place(cuda_device):
             ref.check(rope(q, None, pos, inplace=True)[0], *want, layout)
 
 
+@pytest.mark.parametrize("T", [1, 3, 700])
+def test_rope_many_heads(cuda_device, T):
+    """More heads than a grid dimension holds."""
+    from onecomp_runtime.layers import RotaryEmbedding
+    dev = cuda_device
+    rope, pos = RotaryEmbedding(8), torch.arange(T, device=dev) * 77
+    ang = pos.double()[:, None] * torch.tensor(rope.inv_freq, dtype=torch.float64, device=dev)
+    q, k = randn(dev, T, 70001, 8, seed=1), randn(dev, T, 65536, 8, seed=2)
+    with torch.no_grad():
+        for x, y in zip((q, k), rope(q, k, pos)):
+            ref.check(y, *ref.rope(x, ang, 1.0, 8, False), f"T={T}")
+
+
 # ---------------------------------------------------------------------------------------- dense linear
 @pytest.mark.parametrize("M", [5, 60, 300])
 def test_linear_writes_beside_its_inputs(cuda_device, M):
