@@ -186,6 +186,27 @@ def test_attention_writes_beside_its_inputs(cuda_device, T):
                 packed_attention(q, k, v, out=bad)
 
 
+@pytest.mark.parametrize("D", [8, 64, 128, 256])
+def test_attention_tensors_of_one_row(cuda_device, D):
+    """One query row with many heads (a tile of its own), one key row, one of each, heads kept in other orders: a
+    dimension of one row may have any stride."""
+    from onecomp_runtime.layers import packed_attention
+    dev = cuda_device
+    for Tq, Tk, Hq, Hkv in ((1, 1, 40, 1), (1, 700, 64, 2), (40, 1, 4, 4), (300, 1, 6, 2), (1, 1, 1, 1), (2, 1, 96, 3)):
+        q, k, v = randn(dev, Tq, Hq, D, seed=1), randn(dev, Tk, Hkv, D, seed=2), randn(dev, Tk, Hkv, D, seed=3)
+
+        def other(t):   # heads 3 rows apart, tokens at an odd pitch behind them
+            T, H, _ = t.shape
+            return torch.zeros(H, 3, T, D + 8, dtype=BF, device=dev)[:, 1, :, :D].transpose(0, 1).copy_(t)
+
+        for causal in (True, False):
+            want, tol = ref.attention(q, k, v, [(0, Tq, 0, Tk)], causal, D ** -0.5)
+            with torch.no_grad():
+                ref.check(packed_attention(q, k, v, causal=causal), want, tol, f"{Tq} {Tk}")
+                ref.check(packed_attention(other(q), other(k), other(v), causal=causal, out=other(q)), want, tol, f"{Tq} {Tk} strided")
+    assert error_word(dev) == 0
+
+
 # ---------------------------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("scaling", [None, {"type": "ntk", "factor": 8.0}])
 def test_rope_far_positions_against_long_arithmetic(cuda_device, scaling):
@@ -345,4 +366,45 @@ def test_linear_activations_of_extreme_values(cuda_device, act, dtype, M):
     # the exponent of the fast exponential is off by 2^-16 of the result at most; below the type's normal range one step
     tol = want.abs() * (ref.half_step(dtype) + 2.0 ** -16) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     ref.check(y[fin], want[fin], tol[fin], f"{act}")
+    assert error_word(dev) == 0
+
+
+@pytest.mark.parametrize("M", [1, 20, 40, 300])
+@pytest.mark.parametrize("N", [1, 2, 7, 8, 33])
+def test_linear_few_features(cuda_device, M, N):
+    """Down to one feature and one block of 8 values; a column of a wider output."""
+    from onecomp_runtime.layers import linear_fused
+    dev = cuda_device
+    for K in (8, 72):
+        x, w, b, r = randn(dev, M, K, seed=1), randn(dev, N, K, seed=2), randn(dev, N, seed=3), randn(dev, M, N, seed=4)
+        wide = torch.full((M, N + 4), 7.0, dtype=BF, device=dev)
+        with torch.no_grad():
+            want, tol = ref.linear(x, w, b, "silu", r)
+            ref.check(linear_fused(x, w, b, activation="silu", residual=r), want, tol, f"{M} {N} {K}")
+            ref.check(linear_fused(x, w, b, activation="silu", residual=r, out=wide[:, 2:N + 2]), want, tol, "column")
+        assert bool((wide[:, :2] == 7).all()) and bool((wide[:, N + 2:] == 7).all())
+    assert error_word(dev) == 0
+
+
+def test_operators_under_inference_mode_and_other_streams(cuda_device):
+    """Inference tensors, and tensors made on one stream and used on another after an event."""
+    from onecomp_runtime.layers import RotaryEmbedding, linear_fused, packed_attention
+    dev = cuda_device
+    rope = RotaryEmbedding(64)
+    with torch.inference_mode():
+        x, w = randn(dev, 70, 256, seed=1), randn(dev, 3 * 256, 256, seed=2, std=1 / 16)
+        pos = torch.arange(70, device=dev)
+
+        def step():
+            q, k, v = (t.unflatten(1, (4, 64)) for t in linear_fused(x, w).split(256, 1))
+            rope(q, k, pos, inplace=True)
+            return packed_attention(q, k, v)
+
+        first = step()
+        s = torch.cuda.Stream(dev)
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            second = step()
+        torch.cuda.current_stream(dev).wait_stream(s)
+        assert torch.equal(first, second)
     assert error_word(dev) == 0
