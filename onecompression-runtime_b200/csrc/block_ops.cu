@@ -110,8 +110,10 @@ AttnPlan attn_plan(int Tq, int Tk, int B, int Hq, int Hkv, int D, int max_q, int
   pl.dp = attn_dp(D);
   const int64_t seqs = std::max(B, 1), G = Hq / Hkv;
   const int64_t run = max_q > 0 ? std::min(max_q, Tq) : (Tq + seqs - 1) / seqs;
-  // One tile of 16 (token, head) rows streams the keys from memory at the split kernel's rate; more rows are
-  // tensor work.
+  // One tile of 16 (token, head) rows streams the keys from memory at the split kernel's rate; more rows read them
+  // again there and are tensor work here. 16 sequences of 2048 to 4096 keys in a graph, tile against split kernel:
+  // heads of 128, 32 rows 65.4 and 58.9 us, 48 rows 63.9 and 72.9, 64 rows 65.4 and 112; heads of 64, 32 rows 95.4 and
+  // 87.6, 64 rows 88.0 and 131; heads of 256, 18 rows 57.0 and 62.5, 36 rows 59.2 and 75.2.
   pl.tile = run * G > kTileMinRows && G <= 128 && B > 0 && Tk > 0;
   if (!pl.tile) {
     pl.ctas = split_ctas(pl.dp, sms);
@@ -224,8 +226,10 @@ int launch_dense_split(const void* x, int64_t ldx, const void* w, int64_t ldw, o
 // Tokens of a tile of the K-splitting kernel, or 0 where the pairs take the call.
 // The K-splitting kernel up to 32 tokens, where streaming the weights through every SM decides (one token,
 // weights from HBM, 4096 x 4096: 12.8 us against 16.8 of the pairs; 1024 x 8192: 10.8 against 27.1). Above, the
-// pairs (64 tokens, 2560 x 2560: 13.9 against 11.8), unless few of them would walk a long K (64 tokens,
-// 1024 x 8192: 13.8 against 26.9; 128 tokens: 16.2 against 25.1).
+// pairs (64 tokens, weights in L2: 2560 x 2560 8.5 us against 13.2, 4096 x 4096 11.0 against 15.7), unless few of them
+// would walk a long K (64 tokens, 1024 x 8192 from HBM: 13.8 against 26.9; 128 tokens: 16.2 against 25.1). In between
+// neither wins everywhere (4096 x 8192, pairs and split: 33 tokens 17.0 and 15.1, 64 tokens 17.3 and 18.7, 128 tokens
+// 22.6 and 18.0).
 int dense_split_tokens(int M, int N, int K) {
   const int least_tiles = (N + 255) / 256 * ((M + 31) / 32);   // of the pairs, at 32 tokens each
   if (M <= 16) return 16;
