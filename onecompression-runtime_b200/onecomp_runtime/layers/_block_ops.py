@@ -71,8 +71,9 @@ def overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
     if not (a0 < b1 and b0 < a1):
         return False
     ways_a, ways_b = _rows_of_pitch(a), _rows_of_pitch(b)
-    for pitch in {*ways_a, *ways_b} - {0}:
-        la, lb = ways_a.get(pitch, ways_a[0]), ways_b.get(pitch, ways_b[0])
+    for pitch in {*ways_a, *ways_b} - {0}:   # rows of a multiple of the pitch (or one row) are rows of the pitch too
+        la = min(n for p, n in ways_a.items() if p % pitch == 0)
+        lb = min(n for p, n in ways_b.items() if p % pitch == 0)
         at = (b0 - a0) % pitch
         if la <= at and at + lb <= pitch:
             return False

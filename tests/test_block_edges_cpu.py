@@ -121,11 +121,12 @@ def test_slices_of_one_buffer_share_nothing():
     from onecomp_runtime.layers._block_ops import overlap
     b = zeros(7, 6 * 64)
     q, o = b[:, :128].unflatten(1, (2, 64)), b[:, 256:].unflatten(1, (2, 64))
-    heads = zeros(7, 4, 3, 64)
+    heads, wide = zeros(7, 4, 3, 64), zeros(6, 8, 64)
     batch = zeros(2, 5, 96)
     for x, y in ((q, o), (b[:, :100], b[:, 100:]), (heads[:, :, 0], heads[:, :, 2]), (batch[..., :32], batch[..., 32:]),
                  (b[:3], b[3:]), (b[:, :64], b[2, 64:]), (b[1:, :8], b[:-1, 376:]), (heads[:, 0], heads[:, 1:]),
-                 (heads[:, :, 1, :8], heads[:, :, 1, 8:])):
+                 (heads[:, :, 1, :8], heads[:, :, 1, 8:]), (wide[:, ::2], wide[:, 1:2]), (wide[::2], wide[1:2, 3:]),
+                 (wide[:, ::4], wide[1:3, 2::4])):
         assert not overlap(x, y) and not overlap(y, x) and not addresses(x) & addresses(y)
     for x, y in ((q, b[:, 64:192].unflatten(1, (2, 64))), (b[:, :101], b[:, 100:]), (b[:4], b[3:]), (b, b), (b[:, 64:], b[2, 64:])):
         assert overlap(x, y) and overlap(y, x)
